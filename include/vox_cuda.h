@@ -83,6 +83,8 @@ VOX_CUDA_API int vox_cuda_device_cc(int *cc);
  * with the device). Bit 0 (VOX_CUDA_DEVERR_TIMEOUT): a kernel gave up a bounded wait for its staged data and left
  * its rows unwritten. No counterpart in the reference (Vox's Vulkan backend has no device-side waits). */
 #define VOX_CUDA_DEVERR_TIMEOUT 1u
+/* Bit 1: a paged-cache operator met a length or a page number that is out of range and did not follow it. */
+#define VOX_CUDA_DEVERR_RANGE 2u
 VOX_CUDA_API int vox_cuda_device_error(unsigned int *flags);
 /* Test hook of the row operators (RMSNorm, LayerNorm, adaLN, softmax, row reductions, residual + RMSNorm): from the
  * next launch on, the stage barrier of row `row` (-1 = none) expects 16 bytes more than its copies deliver, so every
@@ -286,6 +288,81 @@ VOX_CUDA_API int vox_cuda_qkv_rope(const float *qkv, const float *q_norm_w, cons
  * rmsnorm.comp (gpu_vulkan.cpp:700-701, 707-708). */
 VOX_CUDA_API int vox_cuda_add_rmsnorm(void *h, const void *delta, const float *layer_scale, const float *w, void *xn, int64_t rows,
                                       int64_t n, float eps, int dtype, void *stream);
+
+/* ---------------------------------------------------------------- paged key/value cache */
+
+/* A paged key/value cache: `pages` pages of `page_size` rows; row r of page p holds, for each key/value head, a key of
+ * head_dim elements at k + p * page_stride + r * row_stride + head * head_stride and a value at the same offset from v.
+ * Pages and rows may lie in any order of memory that these strides give ([pages][page_size][kv_heads][head_dim], or
+ * head-major, or one tensor that holds both); a linear cache is one page a sequence.
+ *   dtype: VOX_CUDA_F32 or VOX_CUDA_BF16; page_size: a power of two, 16 .. 2^20; head_dim: 64 or 128 (the widths of the
+ *   reference's talkers); strides in elements, each a multiple of 16 bytes; k and v 16-byte aligned.
+ * No counterpart in the reference, whose caches are linear or rings of one sequence (appends in transformer_forward,
+ * kernels.cpp:797-806; shaders/ringput.comp). */
+typedef struct vox_cuda_kv_cache {
+    void *k, *v;
+    int32_t dtype, page_size, pages, kv_heads, head_dim;
+    int64_t page_stride, row_stride, head_stride;
+} vox_cuda_kv_cache;
+
+/* A ragged batch over such a cache. All arrays are on the device and are read by the kernels, so a captured graph can be
+ * replayed with other lengths.
+ *   page_table [seqs][table_stride]: the pages of each sequence in order, the first table_width of a row in use
+ *   kv_len     [seqs]: rows of each sequence in the cache, its new tokens included
+ *   q_start    [seqs + 1]: first token of each sequence among the `tokens` rows of qkv / q / out, ascending; or NULL:
+ *              every sequence has tokens / seqs of them
+ *   tokens:    new tokens of all sequences together
+ *   max_q, max_kv: bounds of a sequence's new tokens and of kv_len. They size the launch only: longer sequences are still
+ *              computed whole, more slowly. 0: tokens, and table_width * page_size.
+ * Token i of sequence b stands at position kv_len[b] - q_len[b] + i. Lengths and page numbers are checked on the device:
+ * one that is out of range is never followed, and sets VOX_CUDA_DEVERR_RANGE in vox_cuda_device_error(); the results of that
+ * sequence are then undefined. */
+typedef struct vox_cuda_kv_batch {
+    const int32_t *page_table, *kv_len, *q_start;
+    int64_t table_stride, tokens;
+    int32_t seqs, table_width, max_q, max_kv;
+} vox_cuda_kv_batch;
+
+/* vox_cuda_qkv_rope for a ragged batch and a paged cache: splits the fused projection of every token, head-RMSNorms and
+ * rotates q and k (rotate-half) at the token's position, writes q and the token's K and V rows into its sequence's pages.
+ *   qkv [tokens][heads*hd + 2*kv_heads*hd], row stride qkv_stride elements; q [tokens][heads*hd], row stride q_stride;
+ *   both in `dtype` (f32 or bf16); the cache rows are rounded once to the cache's dtype
+ *   cs: f32 [cs_rows][hd/2][2], the vox_cuda_rope_table of positions 0 .. cs_rows-1 (every position needs its row);
+ *   q_norm_w / k_norm_w: f32 [hd] or NULL; eps their epsilon
+ * Arithmetic as vox_cuda_qkv_rope (with f32 in and out and no head norms bit-identical to rope_apply, kernels.cpp:740-757).
+ * A token whose position has no page or no table row is skipped and sets VOX_CUDA_DEVERR_RANGE. No two tokens
+ * of a call may share a cache row. qkv, q, cs, weights 16-byte aligned, strides multiples of 16 bytes; q must not overlap
+ * qkv. Serves transformer_forward's kernels.cpp:797-806 for a batch. */
+VOX_CUDA_API int vox_cuda_kv_append(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, const void *qkv, int64_t qkv_stride,
+                                    const float *q_norm_w, const float *k_norm_w, const float *cs, int64_t cs_rows, void *q,
+                                    int64_t q_stride, int64_t heads, float eps, int dtype, void *stream);
+
+/* Causal attention of a ragged batch over its paged cache: out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the
+ * rows j of the token's sequence with j <= position (and j > position - window where window > 0), k and v of key/value
+ * head h / (heads / kv_heads). Prompts and single tokens alike (q_len 0, 1 or more a sequence, mixed in a call).
+ *   q, out [tokens][heads][hd], row strides q_stride / out_stride elements, `dtype` f32 or bf16; out must not overlap q
+ * A token that sees no key gives zeros. Cache rows at or past kv_len are never used, whatever they hold; the rows below it
+ * must be finite. f32 activations keep f32 accuracy (CUDA cores). bf16 activations on a bf16 cache run on the tensor cores
+ * with f32 scores, statistics and sums; the weights are rounded to bf16 for the product with v (about 2^-9 relative).
+ * Results are identical run to run. workspace: vox_cuda_attn_workspace bytes of scratch, 256-byte aligned (NULL where that
+ * says 0), not shared by calls that can overlap. Replaces attention.comp:1-45 and the attention of transformer_forward
+ * (kernels.cpp:809-828); window: attnw.comp:1-48. */
+VOX_CUDA_API int vox_cuda_attn_paged(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, const void *q, int64_t q_stride,
+                                     void *out, int64_t out_stride, int64_t heads, float scale, int64_t window, int dtype,
+                                     void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same attention for a batch whose sequences all stand behind one shared prefix (a voice prompt): every token sees the
+ * prefix_len rows behind prefix_pages (device, ceil(prefix_len / page_size) page numbers), then its own sequence's rows as
+ * above (kv_len counts the sequence's own rows). The prefix is read once for the whole batch, not once a sequence; the two
+ * parts' softmax statistics are joined exactly. prefix_len 0 is vox_cuda_attn_paged. */
+VOX_CUDA_API int vox_cuda_attn_prefix(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, const int32_t *prefix_pages,
+                                      int64_t prefix_len, const void *q, int64_t q_stride, void *out, int64_t out_stride,
+                                      int64_t heads, float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that vox_cuda_attn_paged (prefix_len 0) or vox_cuda_attn_prefix needs for this cache and batch shape
+ * (seqs, tokens, max_q, max_kv; the arrays are not read). */
+VOX_CUDA_API int vox_cuda_attn_workspace(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, int64_t prefix_len,
+                                         int64_t heads, int64_t window, int dtype, size_t *bytes);
 
 /* ---------------------------------------------------------------- GEMM on the tensor cores */
 

@@ -23,7 +23,7 @@ __all__ = [
     "rmsnorm", "layernorm", "layer_norm", "adaln", "gated_add", "bias_add",
     "softmax_rows", "silu_mul", "swiglu_fused", "gelu", "add", "mul", "snake", "load_snake",
     "dequant_q8", "dequant_q4", "row_reduce", "global_sum_partials", "global_sum_finish", "global_sum",
-    "fill_philox", "rope_inv_freq", "rope_table", "qkv_rope", "add_rmsnorm", "gemv_q8", "gemv_q4", "gemm_q8", "gemm_q4", "gemm_bf16", "Comm", "global_sum_comm", "Tmod", "F5Dit", "F32", "BF16", "F16",
+    "fill_philox", "rope_inv_freq", "rope_table", "qkv_rope", "add_rmsnorm", "gemv_q8", "gemv_q4", "gemm_q8", "gemm_q4", "gemm_bf16", "Comm", "global_sum_comm", "Tmod", "F5Dit", "PagedKV", "F32", "BF16", "F16",
 ]
 
 F32, BF16, F16 = 0, 1, 2
@@ -88,6 +88,10 @@ def _load() -> ctypes.CDLL:
         "vox_cuda_gemm_q8": ([c_p, c_p, c_int, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_int, c_p], c_int),
         "vox_cuda_gemm_q4": ([c_p, c_p, c_int, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_int, c_p], c_int),
         "vox_cuda_gemm_bf16": ([c_p, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_int, c_int, c_p], c_int),
+        "vox_cuda_kv_append": ([c_p, c_p, c_p, c_i64, c_p, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_f, c_int, c_p], c_int),
+        "vox_cuda_attn_paged": ([c_p, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_f, c_i64, c_int, c_p, ctypes.c_size_t, c_p], c_int),
+        "vox_cuda_attn_prefix": ([c_p, c_p, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_i64, c_f, c_int, c_p, ctypes.c_size_t, c_p], c_int),
+        "vox_cuda_attn_workspace": ([c_p, c_p, c_i64, c_i64, c_i64, c_int, c_p], c_int),
         "vox_cuda_gemv_q8": ([c_p, c_p, c_int, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_int, c_p], c_int),
         "vox_cuda_gemv_q4": ([c_p, c_p, c_int, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_int, c_p], c_int),
         "vox_cuda_tmod_open": ([ctypes.c_char_p, c_p], c_int),
@@ -503,6 +507,155 @@ def add_rmsnorm(h: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: floa
     _check(lib.vox_cuda_add_rmsnorm(h.data_ptr(), delta.data_ptr(), _f32(layer_scale, "layer_scale"), _f32(w, "w"),
                                     out.data_ptr(), h.numel() // n, n, eps, dt, _stream(h)))
     return out
+
+
+# ------------------------------------------------------------------ paged key/value cache
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "page_size", "pages", "kv_heads", "head_dim")] + \
+               [(n, ctypes.c_int64) for n in ("page_stride", "row_stride", "head_stride")]
+
+
+class _KvBatch(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("page_table", "kv_len", "q_start")] + \
+               [(n, ctypes.c_int64) for n in ("table_stride", "tokens")] + \
+               [(n, ctypes.c_int32) for n in ("seqs", "table_width", "max_q", "max_kv")]
+
+
+class PagedKV:
+    """A paged key/value cache of one layer and the operators on it: appending a batch's new tokens (vox_cuda_kv_append)
+    and the attention that reads it (vox_cuda_attn_paged, vox_cuda_attn_prefix).
+
+    `k` and `v` are [pages][page_size][kv_heads][head_dim], f32 or bf16, with equal strides (any order of memory whose
+    last dimension is contiguous: a head-major cache is a permuted view, a linear cache is one page a sequence);
+    page_size a power of two >= 16, head_dim 64 or 128. The tensors stay the caller's; the handle keeps them alive.
+
+    Every call takes a ragged batch: `page_table` int32 [seqs][width] (each sequence's pages in order), `kv_len` int32
+    [seqs] (rows of each sequence with its new tokens), and, unless every sequence has the same number of new tokens,
+    `q_start` int32 [seqs + 1] (first token of each). They are read on the device, on the current stream. A length or
+    page number that is out of range is not followed and sets bit 1 of device_error()."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        for t, nm in ((k, "k"), (v, "v")):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise VoxCudaError(-6, f"{nm} must be a CUDA tensor (vox_b200 has no CPU path)")
+            if t.dim() != 4 or t.dtype not in (torch.float32, torch.bfloat16):
+                raise VoxCudaError(-6, f"{nm} must be float32 or bfloat16 [pages][page_size][kv_heads][head_dim]")
+        _same(k, v, "k", "v")
+        if k.shape != v.shape or k.stride() != v.stride() or k.stride(3) != 1:
+            raise VoxCudaError(-6, "k and v must share shape and strides, the last dimension contiguous")
+        self.k, self.v = k, v
+        self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
+        self._c = _KvCache(k.data_ptr(), v.data_ptr(), F32 if k.dtype == torch.float32 else BF16, self.page_size, self.pages,
+                           self.kv_heads, self.head_dim, *k.stride()[:3])
+        self._cp = ctypes.byref(self._c)
+        self._need = {}  # workspace bytes by batch shape
+
+    def _ints(self, t, name, dims):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.k.device or t.dim() != dims or \
+                (t.shape[-1] > 1 and t.stride(-1) != 1):
+            raise VoxCudaError(-6, f"{name} must be an int32 tensor of {dims} dimension(s) on the cache's device, its last one contiguous")
+        return t.data_ptr()
+
+    def _batch(self, tokens, page_table, kv_len, q_start, max_q, max_kv):
+        pt, pl = self._ints(page_table, "page_table", 2), self._ints(kv_len, "kv_len", 1)
+        ps = None if q_start is None else self._ints(q_start, "q_start", 1)
+        seqs, width = page_table.shape
+        if kv_len.shape[0] != seqs or (q_start is not None and q_start.shape[0] != seqs + 1):
+            raise VoxCudaError(-6, "page_table [seqs][width], kv_len [seqs] and q_start [seqs + 1] must agree")
+        return _KvBatch(pt, pl, ps, page_table.stride(0) if seqs > 1 else width, tokens, seqs, width, max_q, max_kv)
+
+    def _rows(self, t, name, width):
+        """(dtype, tokens, row stride) of activations [tokens][...] whose trailing dimensions are contiguous."""
+        if not isinstance(t, torch.Tensor) or t.device != self.k.device:
+            raise VoxCudaError(-6, f"{name} must be a tensor on the cache's device (vox_b200 has no CPU path)")
+        if t.dim() == 3:
+            ok, inner = t.stride(2) == 1 and (t.stride(1) == t.shape[2] or t.shape[1] == 1), t.shape[1] * t.shape[2]
+        else:
+            ok, inner = t.dim() == 2 and t.stride(1) == 1, t.shape[-1]
+        if not ok or (width and inner != width):
+            raise VoxCudaError(-6, f"{name} must be [tokens][heads * head_dim] or [tokens][heads][head_dim], contiguous within a token"
+                               + (f", {width} elements each" if width else ""))
+        if t.dtype == torch.float32:
+            dt = F32
+        elif t.dtype == torch.bfloat16:
+            dt = BF16
+        else:
+            raise VoxCudaError(-6, f"{name} must be float32 or bfloat16, got {t.dtype}")
+        return dt, t.shape[0], t.stride(0) if t.shape[0] > 1 else inner, inner
+
+    def append(self, qkv, cs, page_table, kv_len, heads: int, q_start=None, q_norm_w=None, k_norm_w=None, eps: float = 1e-6,
+               q=None) -> torch.Tensor:
+        """qkv_rope for a ragged batch: splits the fused projection qkv [tokens][(heads + 2 kv_heads) head_dim], head-
+        RMSNorms and rotates q and k at each token's position, writes K and V into the sequences' pages and returns q
+        [tokens][heads * head_dim] (qkv's dtype). cs: rope_table(inv_freq, 0, n) of all positions in use."""
+        hd = self.head_dim
+        dt, tokens, stride, _ = self._rows(qkv, "qkv", (heads + 2 * self.kv_heads) * hd)
+        if _f32(cs, "cs") and (cs.dim() != 3 or cs.shape[1] != hd // 2 or cs.shape[2] != 2):
+            raise VoxCudaError(-6, "cs must be [positions][head_dim / 2][2]")
+        for w, nm in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+            if w is not None and w.numel() != hd:
+                raise VoxCudaError(-6, f"{nm} must have head_dim elements")
+        if q is None:
+            q = torch.empty((tokens, heads * hd), dtype=qkv.dtype, device=qkv.device)
+        qdt, qtok, qstride, _ = self._rows(q, "q", heads * hd)
+        if qdt != dt or qtok != tokens:
+            raise VoxCudaError(-6, "q must have qkv's dtype and tokens")
+        b = self._batch(tokens, page_table, kv_len, q_start, 0, 0)
+        _check(lib.vox_cuda_kv_append(self._cp, ctypes.byref(b), qkv.data_ptr(), stride, _f32(q_norm_w, "q_norm_w"),
+                                      _f32(k_norm_w, "k_norm_w"), cs.data_ptr(), cs.shape[0], q.data_ptr(), qstride, heads, eps, dt, _stream(qkv)))
+        return q
+
+    def attend(self, q, page_table, kv_len, q_start=None, max_q: int = 0, max_kv: int = 0, scale: float | None = None,
+               window: int = 0, out=None) -> torch.Tensor:
+        """Causal attention of the batch's new tokens over their sequences' cached rows (their own included): q
+        [tokens][heads][head_dim] or [tokens][heads * head_dim] -> the same shape. window > 0: only the last `window`
+        positions. max_q / max_kv: the largest number of new tokens and of rows (host numbers; they size the launch)."""
+        return self._attend(q, None, 0, page_table, kv_len, q_start, max_q, max_kv, scale, window, out)
+
+    def attend_prefix(self, q, prefix_pages, prefix_len: int, page_table, kv_len, q_start=None, max_q: int = 0, max_kv: int = 0,
+                      scale: float | None = None, out=None) -> torch.Tensor:
+        """attend() for sequences that all stand behind one shared prefix: every token sees the prefix_len rows behind
+        prefix_pages (int32), read once for the whole batch, and then its own sequence's rows as in attend()."""
+        self._ints(prefix_pages, "prefix_pages", 1)
+        if not 0 <= prefix_len <= prefix_pages.shape[0] * self.page_size:
+            raise VoxCudaError(-6, "prefix_len must fit prefix_pages")
+        return self._attend(q, prefix_pages, prefix_len, page_table, kv_len, q_start, max_q, max_kv, scale, 0, out)
+
+    def _attend(self, q, prefix_pages, prefix_len, page_table, kv_len, q_start, max_q, max_kv, scale, window, out):
+        hd = self.head_dim
+        dt, tokens, stride, inner = self._rows(q, "q", 0)
+        heads = inner // hd
+        if heads * hd != inner or (q.dim() == 3 and q.shape[2] != hd):
+            raise VoxCudaError(-6, "q must hold whole heads of the cache's head_dim")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        odt, otok, ostride, _ = self._rows(out, "out", inner)
+        if odt != dt or otok != tokens:
+            raise VoxCudaError(-6, "out must have q's dtype and tokens")
+        b = self._batch(tokens, page_table, kv_len, q_start, max_q, max_kv)
+        bp = ctypes.byref(b)
+        key = (b.seqs, tokens, b.table_width, max_q, max_kv, q_start is None, prefix_len, heads, window, dt)
+        need = self._need.get(key)
+        if need is None:
+            n = ctypes.c_size_t()
+            _check(lib.vox_cuda_attn_workspace(self._cp, bp, prefix_len, heads, window, dt, ctypes.byref(n)))
+            if len(self._need) > 4096:
+                self._need.clear()
+            need = self._need[key] = n.value
+        # scratch of this call alone, from torch's allocator: it is reused only behind this call on the same stream
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        if scale is None:
+            scale = hd ** -0.5
+        if prefix_pages is None:
+            rc = lib.vox_cuda_attn_paged(self._cp, bp, q.data_ptr(), stride, out.data_ptr(), ostride, heads, scale, window, dt,
+                                         None if ws is None else ws.data_ptr(), need, _stream(q))
+        else:
+            rc = lib.vox_cuda_attn_prefix(self._cp, bp, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), stride, out.data_ptr(), ostride,
+                                          heads, scale, dt, None if ws is None else ws.data_ptr(), need, _stream(q))
+        _check(rc)
+        return out
 
 
 # ------------------------------------------------------------------ GEMM on the tensor cores

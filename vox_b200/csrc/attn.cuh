@@ -1,0 +1,85 @@
+// Internal interface of the paged attention kernels: their arguments, the split of a call into jobs, and the launchers.
+//
+// One call is a list of jobs (rows x keys of one key/value head): the rows are query heads of tokens that share that head,
+// the keys a range of one sequence's cache or of the shared prefix. A range that one block takes alone is normalised and
+// stored at once; a range cut into splits leaves for each row and split the running maximum and sum of its softmax (f32)
+// and the unnormalised output (f32) in the workspace, and attn_merge joins the splits of a row in ascending order:
+//   M = max_s m_s,  out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s
+// (all exponents base 2: the scores are scaled by scale * log2 e before the softmax).
+#pragma once
+
+#include "paged.cuh"
+
+namespace voxcuda {
+
+struct AttnArgs {
+    PagedArgs p;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;  // elements
+    const int32_t *prefix_pages;
+    int32_t prefix_len, window;    // window 0: none
+    float scale_log2;              // scale * log2 e
+    FastDiv gdiv;                  // division by p.group
+    // the own keys of a sequence: split s takes keys [s * chunk, (s + 1) * chunk), chunk at least own_chunk
+    int32_t own_splits, own_chunk, own_tiles;  // tiles: blocks over the rows of a sequence
+    // the prefix: likewise, over the rows of all tokens
+    int32_t pre_splits, pre_chunk, pre_tiles;
+    FastDiv kvdiv, otdiv, osdiv, ptdiv;        // divisions by kv_heads, own_tiles, own_splits, pre_tiles
+    int32_t pre_blocks, splits;                // blocks of the prefix (they come first); pre_splits + own_splits
+    float *part_o;                             // [tokens * heads][splits][hd], splits > 1
+    float2 *part_ml;                           // [tokens * heads][splits]: (maximum, sum)
+};
+
+// A block's job, the same in every kernel.
+struct AttnJob {
+    int tok0, rows;        // first token; rows = tokens of the job * group
+    int kvh;
+    int split;             // slot of the partial results
+    int base;              // causal: row of token i sees keys < base + i + 1 (own keys); prefix: every key
+    bool causal;
+    int k0, k1;            // keys of the split
+    const int32_t *pages;  // page numbers of the keys
+    int tile, tiles;       // row tiles: tile, tile + tiles, ...
+};
+
+__device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
+    AttnJob j;
+    uint32_t x = blk;
+    if (blk < uint32_t(a.pre_blocks)) {
+        const uint32_t y = a.kvdiv.div(x);
+        j.kvh = int(x - y * uint32_t(a.p.kv_heads));
+        j.split = int(a.ptdiv.div(y));
+        j.tile = int(y - uint32_t(j.split) * uint32_t(a.pre_tiles));
+        j.tiles = a.pre_tiles;
+        j.tok0 = 0, j.rows = a.p.tokens * a.p.group;
+        j.base = 0, j.causal = false;
+        j.pages = a.prefix_pages;
+        j.k0 = min(j.split * a.pre_chunk, a.prefix_len);
+        j.k1 = j.split + 1 == a.pre_splits ? a.prefix_len : min(j.k0 + a.pre_chunk, a.prefix_len);
+        return j;
+    }
+    x -= uint32_t(a.pre_blocks);
+    uint32_t y = a.kvdiv.div(x);
+    j.kvh = int(x - y * uint32_t(a.p.kv_heads));
+    uint32_t z = a.otdiv.div(y);
+    j.tile = int(y - z * uint32_t(a.own_tiles));
+    j.tiles = a.own_tiles;
+    const uint32_t b = a.osdiv.div(z);
+    const int s = int(z - b * uint32_t(a.own_splits));
+    j.split = a.pre_splits + s;
+    int n;
+    seq_tokens(a.p, int(b), j.tok0, n);
+    const int kv = seq_rows(a.p, int(b));
+    j.rows = n * a.p.group;
+    j.base = kv - n, j.causal = true;
+    j.pages = a.p.table + int64_t(b) * a.p.table_stride;
+    // a sequence longer than the host's bound gets longer splits, whole tiles of 128 keys
+    const int chunk = max(a.own_chunk, ((kv + a.own_splits - 1) / a.own_splits + 127) & ~127);
+    j.k0 = int(min(int64_t(s) * chunk, int64_t(kv)));
+    j.k1 = int(min(int64_t(j.k0) + chunk, int64_t(kv)));
+    return j;
+}
+
+
+}  // namespace voxcuda

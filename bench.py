@@ -547,7 +547,8 @@ class CpuSuite:
             Q = P.L
             x3f, r3f, sh3f, sc3f, g3f, y3f = wide(x3), wide(r3), wide(sh3), wide(sc3), wide(g3), E(8, 2048, 1024)
             a6f, b6f, y6f = wide(a6), wide(b6), E(rows, 4096)
-            self._keep += [x3f, r3f, sh3f, sc3f, g3f, y3f, a6f, b6f, y6f]
+            rr = np.empty(rows, np.float64)  # the restatement's row results are f64
+            self._keep += [x3f, r3f, sh3f, sc3f, g3f, y3f, a6f, b6f, y6f, rr]
             add("cfg1_rmsnorm_f32", lambda: Q.vo_rmsnorm_rows(pt(x1), pt(w1), 512, 1024, 1e-6, pt(y1)))
             add("cfg1_swiglu_f32", lambda: Q.vo_silu_mul(pt(g1), pt(u1), pt(h1), g1.size))
             add("cfg2_softmax_causal_f32", lambda: Q.vo_softmax_rows(pt(s2), pt(p2), 16 * 1024, 1024, sc2, 1024, 0))

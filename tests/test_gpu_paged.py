@@ -96,7 +96,7 @@ def attention64(bt, q, heads, scale, window=0):
                 continue
             qi = q[at + i].double().view(bt.kvh, grp, bt.hd)
             s = torch.einsum("hgd,nhd->hgn", qi, kk) * scale
-            big = max(big, float((torch.einsum("hgd,nhd->hgn", qi.abs(), kk.abs()) * scale).max()))
+            big = max(big, float((torch.einsum("hgd,nhd->hgn", qi.abs(), kk.abs()) * abs(scale)).max()))
             w = torch.softmax(s, -1)
             out[at + i] = torch.einsum("hgn,nhd->hgd", w, vv).reshape(heads, bt.hd)
             mag[at + i] = torch.einsum("hgn,nhd->hgd", w, vv.abs()).reshape(heads, bt.hd)
@@ -152,6 +152,19 @@ def test_attend_window(vox, act, cache, window):
     got = bt.handle(vox).attend(q.cuda(), table, kv_len, q_start=q_start, window=window)
     want, mag, big = attention64(bt, q, 6, 64 ** -0.5, window)
     check(got, want, mag, big, act, cache, 300)
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 0.5])
+def test_attend_scale(vox, act, cache, scale):
+    """Any scale: negative, zero (the mean of the values seen), large."""
+    lens = [(1, 200), (50, 150), (3, 3)]
+    bt = Batch(lens, 2, 64, 16, cache, seed=8)
+    q = queries(bt, 4, act)
+    table, kv_len, q_start = bt.dev()
+    got = bt.handle(vox).attend(q.cuda(), table, kv_len, q_start=q_start, scale=scale)
+    want, mag, big = attention64(bt, q, 4, scale)
+    check(got, want, mag, big, act, cache, 200)
 
 
 @pytest.mark.parametrize("act,cache", KINDS, ids=IDS)

@@ -1,5 +1,7 @@
 // Attention over a paged key/value cache: vox_cuda_attn_paged and vox_cuda_attn_prefix, their split of the work, the
 // CUDA-core kernel (every type, exact to f32) and the join of split rows.
+#include <cmath>
+
 #include "attn.cuh"
 #include "sfu.cuh"
 
@@ -209,15 +211,16 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const AttnArgs a) {
 
 int ceil_div(int64_t x, int64_t y) { return int((x + y - 1) / y); }
 
-// How a call is cut: rows a block (R), row tiles, key splits.
+// How a call is cut: which kernels take its parts, rows a block, row tiles, key splits.
 struct AttnShape {
-    int rows_blk;
+    bool own_tc, pre_tc, concat;
+    int rows_blk, tc_rows;
     int own_tiles, own_splits, own_chunk;
     int pre_tiles, pre_splits, pre_chunk;
-    int64_t blocks;
+    int64_t own_blocks, pre_blocks;
 };
 
-// Keys cut into `splits` of whole 128-key tiles.
+// Keys cut into at most `want` splits of whole 128-key tiles.
 void cut_keys(int64_t keys, int64_t want, int &splits, int &chunk) {
     const int64_t tiles = keys > 0 ? (keys + 127) / 128 : 1;
     int64_t n = want < 1 ? 1 : want > tiles ? tiles : want;
@@ -226,20 +229,33 @@ void cut_keys(int64_t keys, int64_t want, int &splits, int &chunk) {
     chunk = int(per * 128);
 }
 
-AttnShape attn_shape(const PagedArgs &p, int64_t max_q, int64_t max_kv, int64_t prefix_len) {
+AttnShape attn_shape(const PagedArgs &p, int64_t max_q, int64_t max_kv, int64_t prefix_len, bool tc_types) {
     AttnShape s = {};
-    const int64_t rows = max_q * p.group;
+    const int64_t rows = max_q * p.group, all = int64_t(p.tokens) * p.group, sms = sm_count();
     s.rows_blk = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
-    s.own_tiles = ceil_div(rows > 0 ? rows : 1, s.rows_blk);
-    const int64_t target = int64_t(sm_count()) * 4;
-    const int64_t own = int64_t(p.seqs) * p.kv_heads * s.own_tiles;
-    cut_keys(max_kv, ceil_div(target, own), s.own_splits, s.own_chunk);
-    s.blocks = own * s.own_splits;
-    if (prefix_len > 0) {
-        s.pre_tiles = ceil_div(int64_t(p.tokens) * p.group, s.rows_blk);
+    s.own_tc = tc_types && rows > 16;
+    s.pre_tc = tc_types && all > 16;
+    s.concat = prefix_len > 0 && s.own_tc && rows >= 64;
+    if (s.own_tc) {
+        // row tiles of all sequences together: exact for equal counts, else one more a sequence at most
+        auto tiles = [&](int64_t rb) { return p.q_start ? all / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
+        s.tc_rows = tiles(256) * p.kv_heads >= sms / 2 ? 256 : 128;
+        s.own_tiles = int(tiles(s.tc_rows));
+        const int64_t own = int64_t(s.own_tiles) * p.kv_heads;
+        cut_keys(max_kv, s.concat ? 1 : own < sms ? sms / own : 1, s.own_splits, s.own_chunk);
+        s.own_blocks = own * s.own_splits;
+    } else {
+        s.own_tiles = ceil_div(rows > 0 ? rows : 1, s.rows_blk);
+        const int64_t own = int64_t(p.seqs) * p.kv_heads * s.own_tiles;
+        cut_keys(max_kv, ceil_div(sms * 4, own), s.own_splits, s.own_chunk);
+        s.own_blocks = own * s.own_splits;
+    }
+    if (prefix_len > 0 && !s.concat) {
+        if (s.pre_tc) s.tc_rows = all > 128 ? 256 : 128;
+        s.pre_tiles = ceil_div(all, s.pre_tc ? s.tc_rows : s.rows_blk);
         const int64_t pre = int64_t(p.kv_heads) * s.pre_tiles;
-        cut_keys(prefix_len, ceil_div(target, pre), s.pre_splits, s.pre_chunk);
-        s.blocks += pre * s.pre_splits;
+        cut_keys(prefix_len, s.pre_tc ? (pre < sms ? sms / pre : 1) : ceil_div(sms * 4, pre), s.pre_splits, s.pre_chunk);
+        s.pre_blocks = pre * s.pre_splits;
     }
     return s;
 }
@@ -252,12 +268,12 @@ size_t workspace_of(const PagedArgs &p, const AttnShape &s, int head_dim) {
 }
 
 template <typename QT, typename CT, int HD>
-int launch_vec(const AttnArgs &a, const AttnShape &s, cudaStream_t st, const char *name) {
+int launch_vec(const AttnArgs &a, const AttnShape &s, int64_t blocks, cudaStream_t st, const char *name) {
     auto kern = s.rows_blk == 1   ? attn_vec_kernel<QT, CT, HD, 1>
                 : s.rows_blk == 2 ? attn_vec_kernel<QT, CT, HD, 2>
                 : s.rows_blk == 4 ? attn_vec_kernel<QT, CT, HD, 4>
                                   : attn_vec_kernel<QT, CT, HD, 8>;
-    launch_k(kern, dim3(unsigned(s.blocks)), kVecThreads, 0, st, a);
+    launch_k(kern, dim3(unsigned(blocks)), kVecThreads, 0, st, a);
     return check_launch(name);
 }
 
@@ -282,8 +298,9 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     const int hd = cache->head_dim;
     const int64_t max_q = batch->q_start == nullptr ? a.p.q_per : batch->max_q > 0 && batch->max_q < batch->tokens ? batch->max_q : batch->tokens;
     const int64_t max_kv = batch->max_kv > 0 && batch->max_kv < a.p.cap ? batch->max_kv : a.p.cap;
-    const AttnShape s = attn_shape(a.p, max_q, max_kv, prefix_len);
-    VOX_REQUIRE(s.blocks < (int64_t(1) << 31), nm + ": sizes out of range");
+    const bool tc_types = dtype == VOX_CUDA_BF16 && cache->dtype == VOX_CUDA_BF16;
+    const AttnShape s = attn_shape(a.p, max_q, max_kv, prefix_len, tc_types);
+    VOX_REQUIRE(s.own_blocks + s.pre_blocks < (int64_t(1) << 31), nm + ": sizes out of range");
     const size_t need = workspace_of(a.p, s, hd);
     if (want) {
         *want = need;
@@ -306,20 +323,34 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.kvdiv = FastDiv(uint32_t(a.p.kv_heads)), a.otdiv = FastDiv(uint32_t(s.own_tiles)), a.osdiv = FastDiv(uint32_t(s.own_splits));
     a.ptdiv = FastDiv(uint32_t(s.pre_tiles > 0 ? s.pre_tiles : 1));
     a.splits = s.own_splits + s.pre_splits;
-    a.pre_blocks = s.pre_splits * s.pre_tiles * a.p.kv_heads;
+    a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
+    a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;
+    a.tc_rows = s.tc_rows, a.concat = s.concat;
     const size_t slots = size_t(a.p.tokens) * size_t(heads) * size_t(a.splits);
     a.part_o = static_cast<float *>(workspace);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + slots * size_t(hd) * sizeof(float));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     using bf = __nv_bfloat16;
     const bool qf = dtype == VOX_CUDA_F32, cf = cache->dtype == VOX_CUDA_F32;
-    int r;
-    if (hd == 64)
-        r = qf ? (cf ? launch_vec<float, float, 64>(a, s, st, name) : launch_vec<float, bf, 64>(a, s, st, name))
-               : (cf ? launch_vec<bf, float, 64>(a, s, st, name) : launch_vec<bf, bf, 64>(a, s, st, name));
-    else
-        r = qf ? (cf ? launch_vec<float, float, 128>(a, s, st, name) : launch_vec<float, bf, 128>(a, s, st, name))
-               : (cf ? launch_vec<bf, float, 128>(a, s, st, name) : launch_vec<bf, bf, 128>(a, s, st, name));
+    int r = VOX_CUDA_OK;
+    if (s.pre_blocks > 0 && s.pre_tc) {
+        a.tc_prefix = 1;
+        r = attn_tc_launch(a, *cache, s.pre_blocks, st, name);
+        a.tc_prefix = 0;
+        if (r != VOX_CUDA_OK) return r;
+    }
+    if (s.own_tc) {
+        r = attn_tc_launch(a, *cache, s.own_blocks, st, name);
+    } else {
+        a.pre_blocks = s.pre_tc ? 0 : int32_t(s.pre_blocks);
+        const int64_t n = a.pre_blocks + s.own_blocks;
+        if (hd == 64)
+            r = qf ? (cf ? launch_vec<float, float, 64>(a, s, n, st, name) : launch_vec<float, bf, 64>(a, s, n, st, name))
+                   : (cf ? launch_vec<bf, float, 64>(a, s, n, st, name) : launch_vec<bf, bf, 64>(a, s, n, st, name));
+        else
+            r = qf ? (cf ? launch_vec<float, float, 128>(a, s, n, st, name) : launch_vec<float, bf, 128>(a, s, n, st, name))
+                   : (cf ? launch_vec<bf, float, 128>(a, s, n, st, name) : launch_vec<bf, bf, 128>(a, s, n, st, name));
+    }
     if (r != VOX_CUDA_OK || a.splits == 1) return r;
     if (hd == 64) return qf ? launch_merge<float, 64>(a, st, name) : launch_merge<bf, 64>(a, st, name);
     return qf ? launch_merge<float, 128>(a, st, name) : launch_merge<bf, 128>(a, st, name);

@@ -27,6 +27,12 @@ struct AttnArgs {
     int32_t pre_splits, pre_chunk, pre_tiles;
     FastDiv kvdiv, otdiv, osdiv, ptdiv;        // divisions by kv_heads, own_tiles, own_splits, pre_tiles
     int32_t pre_blocks, splits;                // blocks of the prefix (they come first); pre_splits + own_splits
+    // the tensor-core kernel: rows a block; whether this launch takes the prefix; whether the own keys follow the prefix
+    // in one walk (then pre_splits is 0). own_tiles counts the row tiles of all sequences there.
+    int32_t tc_rows, tc_prefix, concat;
+    // there the scale is positive (row maxima are taken before it): a negative one flips q's signs, zero clears q
+    float tc_scale;
+    uint32_t q_and, q_xor;
     float *part_o;                             // [tokens * heads][splits][hd], splits > 1
     float2 *part_ml;                           // [tokens * heads][splits]: (maximum, sum)
 };
@@ -81,5 +87,8 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
     return j;
 }
 
+
+// The tensor-core path (attn_tc.cu).
+int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name);
 
 }  // namespace voxcuda

@@ -1,0 +1,476 @@
+// The paged attention of many query rows on the 5th-generation tensor cores (bf16 activations on a bf16 cache).
+//
+// A block takes up to two tiles of 128 query rows of one key/value head (row = token * group + query head in the group, so
+// the heads that share keys share every tile of K and V) and walks the keys in tiles of 128: S = Q K^T (M 128, N 128 keys)
+// and O += P V (M 128, N hd), both accumulated in f32 in tensor memory; P (bf16) overwrites the upper half of its S
+// columns, from where the second product reads it as its A operand. TMEM: S0 S1 at columns 0 and 128, O0 O1 at 256.
+//   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row. Online softmax with a lazy reference: the row's reference
+//                   maximum moves only when a score exceeds it by 8 (in powers of two: weights stay below 256, far from
+//                   any overflow), so O is rescaled in the few tiles where it does; exact, since numerator and
+//                   denominator always share the reference.
+//   warp 8          tensor copies of K and V tiles through a ring of stages, page by page (a box never leaves a page);
+//                   rows of V past the last key are zeroed (their weight is 0, and 0 times what lies there may be NaN)
+//   warp 9          issues the MMAs (warps 10 and 11 only complete the warpgroup that gives its registers away): P V of a tile, then Q K^T of the next tile of the same rows, alternating between the
+//                   two row tiles, so that one tile's softmax runs while the other's products do.
+// Tile order in the ring: K0 V0 K1 V1 ... (both row tiles read each). Every wait is bounded.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "attn.cuh"
+#include "sfu.cuh"
+#include "tc.cuh"
+
+namespace voxcuda {
+namespace {
+
+constexpr int kKeys = 128;
+constexpr int kTcThreads = 384;
+constexpr int kTcRegs = 168;  // registers a thread at launch; 2 x 224 + 56 = 3 x 168 after the split below
+constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
+
+constexpr int tc_stages(int hd) { return hd == 128 ? 5 : 8; }
+constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }
+
+// D[tmem] (+)= A[tmem] . B[smem], issued by one elected lane of a converged warp (A: 128 lanes, two bf16 a column).
+__device__ __forceinline__ void umma_bf16_ta_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 16 consecutive columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Tiled tensor copy of a 4-D map's box; x times the element size is a multiple of 128 bytes at every call site.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+struct TcJob {
+    int ok;
+    int tok0, rows, row0;  // tokens of the job start at tok0; this block's rows row0 .. of `rows`
+    int kvh, split;
+    int base, causal;
+    int pa0, pa1;          // keys of the shared prefix
+    int k0, k1;            // own keys
+    const int32_t *pages;  // of the own keys
+};
+
+// The job of block `blk`, found by warp 0 (every lane takes part).
+__device__ __forceinline__ void tc_job(const AttnArgs &a, uint32_t blk, TcJob &out) {
+    const int lane = threadIdx.x & 31;
+    TcJob j = {};
+    uint32_t y = a.kvdiv.div(blk);
+    j.kvh = int(blk - y * uint32_t(a.p.kv_heads));
+    if (a.tc_prefix) {  // rows of all tokens against a split of the prefix
+        const uint32_t s = a.ptdiv.div(y);
+        j.row0 = int(y - s * uint32_t(a.pre_tiles)) * a.tc_rows;
+        j.rows = a.p.tokens * a.p.group;
+        j.split = int(s);
+        j.pa0 = min(int(s) * a.pre_chunk, a.prefix_len);
+        j.pa1 = int(s) + 1 == a.pre_splits ? a.prefix_len : min(j.pa0 + a.pre_chunk, a.prefix_len);
+        j.ok = j.row0 < j.rows;
+    } else {
+        const uint32_t t0 = a.osdiv.div(y);
+        const int s = int(y - t0 * uint32_t(a.own_splits));
+        int t = a.own_tiles - 1 - int(t0), b = -1, n = 0, tile = 0;  // the last rows, which see most keys, first
+        if (a.p.q_start == nullptr) {
+            const int per = (a.p.q_per * a.p.group + a.tc_rows - 1) / a.tc_rows;
+            b = t / per;
+            tile = t - b * per;
+            j.tok0 = b * a.p.q_per, n = a.p.q_per;
+        } else {
+            for (int c = 0; c < a.p.seqs; c += 32) {
+                int tk = 0, m = 0;
+                if (c + lane < a.p.seqs) seq_tokens(a.p, c + lane, tk, m);
+                const int mine = int((int64_t(m) * a.p.group + a.tc_rows - 1) / a.tc_rows);
+                int cum = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, cum, o);
+                    if (lane >= o) cum += v;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, cum > t);
+                if (hit) {
+                    const int l = __ffs(int(hit)) - 1;
+                    b = c + l;
+                    j.tok0 = __shfl_sync(0xffffffffu, tk, l), n = __shfl_sync(0xffffffffu, m, l);
+                    tile = t - __shfl_sync(0xffffffffu, cum - mine, l);
+                    break;
+                }
+                t -= __shfl_sync(0xffffffffu, cum, 31);
+            }
+        }
+        if (b >= 0) {
+            const int kv = seq_rows(a.p, b);
+            j.rows = n * a.p.group, j.row0 = tile * a.tc_rows;
+            j.base = kv - n, j.causal = 1;
+            j.split = (a.concat ? 0 : a.pre_splits) + s;
+            j.pages = a.p.table + int64_t(b) * a.p.table_stride;
+            const int chunk = max(a.own_chunk, ((kv + a.own_splits - 1) / a.own_splits + 127) & ~127);
+            j.k0 = int(min(int64_t(s) * chunk, int64_t(kv)));
+            j.k1 = int(min(int64_t(j.k0) + chunk, int64_t(kv)));
+            if (a.concat) j.pa1 = a.prefix_len;  // the prefix stands in front of the own keys (one split)
+            j.ok = j.row0 < j.rows;
+        }
+    }
+    if (lane == 0) out = j;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+    constexpr int NS = tc_stages(HD), H = HD / 64;
+    constexpr uint32_t kTile = H * kHalf;
+    constexpr uint32_t kIdS = umma_idesc_bf16(128, kKeys), kIdO = umma_idesc_bf16(128, HD, true);
+    extern __shared__ uint8_t raw[];
+    __shared__ TcJob job;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sQ = smem_addr(smem), sKV = sQ + 2 * kTile;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + (2 + NS) * kTile), *empty = full + NS;
+    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *tail = o_full + 2, *drain = tail + 1;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_enter();
+    if (warp == 0) tc_job(a, blockIdx.x, job);
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int q = 0; q < 2; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 128), mbar_init(&o_full[q], 1);
+        mbar_init(tail, 1);
+        mbar_init(drain, 1);
+        mbar_init_fence();
+    }
+    __syncthreads();
+    const TcJob j = job;
+    if (!j.ok) return;
+    if (warp == 9) tmem_alloc(tslot, 512);
+    // key tiles: nA of the prefix, then the own keys from kb0; hi of a row tile = keys that its last row sees
+    const int nA = (j.pa1 - j.pa0 + kKeys - 1) / kKeys;
+    int kb0 = j.k0;
+    if (a.window > 0 && j.causal) {
+        const int first = int(a.gdiv.div(uint32_t(j.row0)));
+        kb0 = max(kb0, max(j.base + first + 1 - a.window, 0) & ~(kKeys - 1));
+    }
+    int nt[2], kend = 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int r0 = j.row0 + 128 * q;
+        nt[q] = 0;
+        if (r0 < j.rows && 128 * q < a.tc_rows) {
+            const int last = int(a.gdiv.div(uint32_t(min(r0 + 127, j.rows - 1))));
+            const int hi = j.causal ? min(j.base + last + 1, j.k1) : 0;
+            nt[q] = nA + max(hi - kb0 + kKeys - 1, 0) / kKeys;
+            kend = max(kend, hi);
+        }
+    }
+    const int nmax = max(nt[0], nt[1]);
+    if (warp < 8) {  // Q tiles: 16-byte chunks of whole rows, 128-byte swizzle; rows past the end are zero
+        const int q = warp >> 2, w = warp & 3;
+        const uint32_t tQ = sQ + q * kTile;
+        constexpr int CH = HD / 8, RPI = 32 / CH;  // chunks a row, rows a warp step
+#pragma unroll 4
+        for (int s = 0; s < 32 / RPI; ++s) {
+            const int r = w * 32 + s * RPI + lane / CH, c = lane % CH, rr = j.row0 + 128 * q + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (rr < j.rows && nt[q] > 0) {
+                const int i = int(a.gdiv.div(uint32_t(rr))), h = j.kvh * a.p.group + rr - i * a.p.group;
+                v = ld_stream(static_cast<const __nv_bfloat16 *>(a.q) + int64_t(j.tok0 + i) * a.q_stride + int64_t(h) * HD + c * 8);
+            }
+            v.x = (v.x & a.q_and) ^ a.q_xor, v.y = (v.y & a.q_and) ^ a.q_xor, v.z = (v.z & a.q_and) ^ a.q_xor, v.w = (v.w & a.q_and) ^ a.q_xor;
+            const uint32_t dst = tQ + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        fence_proxy_async();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tslot;
+
+    if (warp < 8) {
+        // ---------------------------------------------------------------- softmax: thread = row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int q = warp >> 2, row = (warp & 3) * 32 + lane, rr = j.row0 + 128 * q + row;
+        const int n = q ? nt[1] : nt[0];
+        const uint32_t tS = tmem + (uint32_t((warp & 3) * 32) << 16) + 128 * q, tP = tS + 64;
+        const uint32_t tO = tmem + (uint32_t((warp & 3) * 32) << 16) + 256 + HD * q;
+        const bool live = rr < j.rows && 128 * q < a.tc_rows;
+        const int i_tok = int(a.gdiv.div(uint32_t(live ? rr : 0)));
+        const int hi_own = live && j.causal ? min(j.base + i_tok + 1, j.k1) : 0;
+        const int lo_own = a.window > 0 ? max(j.base + i_tok + 1 - a.window, j.k0) : j.k0;
+        float ref = -INFINITY;  // reference maximum (scaled, base 2)
+        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            ok = mbar_wait_warp(&s_full[q], uint32_t(i & 1));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t r[128];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
+            const bool pre = i < nA;
+            const int key0 = pre ? j.pa0 + i * kKeys : kb0 + (i - nA) * kKeys;
+            const int hi = (pre ? (live ? j.pa1 : 0) : hi_own) - key0, lo = (pre ? j.pa0 : lo_own) - key0;
+            if (!__all_sync(0xffffffffu, hi >= kKeys && lo <= 0)) {
+#pragma unroll
+                for (int c = 0; c < kKeys; ++c)
+                    if (c >= hi || c < lo) r[c] = __float_as_uint(-INFINITY);
+            }
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kKeys; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(r[c]));
+            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.tc_scale;
+            const bool move = mx > ref + 8.0f;  // also the first key that the row sees (ref = -inf)
+            if (__any_sync(0xffffffffu, move)) {
+                const float nref = move ? mx : ref;
+                const float alpha = move ? ex2_approx(ref - nref) : 1.0f;
+                ref = nref;
+                l2[0] = mul2(l2[0], bc2(alpha)), l2[1] = mul2(l2[1], bc2(alpha));
+                if (i > 0) {  // the arrival of this S implies that the P V before it has completed
+#pragma unroll
+                    for (int c = 0; c < HD / 16; ++c) {
+                        uint32_t o[16];
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                                     : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
+                                       "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                                     : "r"(tO + 16 * c)
+                                     : "memory");
+                        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                                     : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]), "+r"(o[8]),
+                                       "+r"(o[9]), "+r"(o[10]), "+r"(o[11]), "+r"(o[12]), "+r"(o[13]), "+r"(o[14]), "+r"(o[15])
+                                     :
+                                     : "memory");
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st16(tO + 16 * c, o);
+                    }
+                }
+            }
+            const float2 sc = bc2(a.tc_scale), nr = bc2(ref == -INFINITY ? 0.f : -ref);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int k = 32 * c + 2 * e;
+                    const float2 x = fma2(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc, nr);
+                    const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    l2[e & 1] = add2(l2[e & 1], p);
+                    w[e] = pack_bf16(p.x, p.y);
+                }
+                tmem_st16(tP + 16 * c, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[q]);
+        }
+        if (n > 0 && ok) {
+            ok = mbar_wait_warp(&o_full[q], 0);
+            tc_fence_after();
+        }
+        const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+        const int h = j.kvh * a.p.group + (live ? rr - i_tok * a.p.group : 0);
+        const int64_t tok = j.tok0 + i_tok;
+        const int64_t slot = (tok * a.p.heads + h) * a.splits + j.split;
+        const float inv = a.splits > 1 ? 1.0f : l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
+        __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + tok * a.out_stride + int64_t(h) * HD;
+        float *pdst = a.part_o + slot * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            if (n > 0 && ok) {
+                tmem_ld32(tO + 32 * c, o);
+                tmem_wait_ld(o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if (!live || !ok) continue;
+            if (a.splits > 1) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<uint4 *>(pdst + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    float f[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(o[e + u]) * inv;
+                    *reinterpret_cast<uint4 *>(dst + 32 * c + e) = Vec<VOX_CUDA_BF16>::pack(f);
+                }
+            }
+        }
+        if (live && ok && a.splits > 1) a.part_ml[slot] = make_float2(ref, l);
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
+        // ---------------------------------------------------------------- copies
+        const int pr = min(a.p.page_mask + 1, kKeys);  // rows a box
+        bool ok = true;
+        int tails = 0, n = 0;
+        for (; n < 2 * nmax && ok; ++n) {
+            const int i = n >> 1, s = n % NS;
+            const bool is_v = n & 1, pre = i < nA;
+            const int key0 = pre ? j.pa0 + i * kKeys : kb0 + (i - nA) * kKeys;
+            const int valid = min((pre ? j.pa1 : kend) - key0, kKeys);
+            if (n >= NS) ok = mbar_wait_warp(&empty[s], uint32_t(n / NS - 1) & 1u);
+            if (!ok) break;
+            const int boxes = (valid + pr - 1) / pr * H;
+            const bool zero = is_v && valid < kKeys;
+            uint64_t *bar = zero ? tail : &full[s];
+            const uint32_t st = sKV + s * kTile;
+            if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(boxes * pr) * 128u);
+            __syncwarp();
+            if (lane < boxes) {
+                const int p = lane / H, half = lane % H, key = key0 + p * pr;
+                const int page = page_checked(a.p, __ldg((pre ? a.prefix_pages : j.pages) + (key >> a.p.page_shift)));
+                tma_load_4d(st + half * kHalf + p * pr * 128, is_v ? &mv : &mk, half * 64, j.kvh, key & a.p.page_mask, page, bar);
+            }
+            if (zero) {
+                ok = mbar_wait_warp(tail, uint32_t(tails++ & 1));
+                for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
+#pragma unroll
+                    for (int half = 0; half < H; ++half)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(st + half * kHalf + x * 16), "r"(0) : "memory");
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+            }
+        }
+        // every copy issued has landed before the block's shared memory is released
+        for (int m = max(n - NS, 0); m < n; ++m) mbar_wait_warp(&full[m % NS], uint32_t(m / NS) & 1u);
+    } else if (warp == 9) {
+        // ---------------------------------------------------------------- MMAs
+        bool ok = true;
+        auto wait_full = [&](int m) { return mbar_wait_warp(&full[m % NS], uint32_t(m / NS) & 1u); };
+        auto qk = [&](int q, int m) {
+            const uint32_t tQ = sQ + q * kTile, tK = sKV + (m % NS) * kTile;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
+                umma_bf16_warp(tmem + 128 * q, umma_desc(tQ + off, 16, 1024), umma_desc(tK + off, 16, 1024), kIdS, k > 0);
+            }
+            umma_commit_warp(&s_full[q]);
+        };
+        if (nmax > 0) {
+            ok = wait_full(0);
+            tc_fence_after();
+            if (ok) {
+                for (int q = 0; q < 2; ++q)
+                    if (nt[q] > 0) qk(q, 0);
+                umma_commit_warp(&empty[0]);
+            }
+        }
+        for (int i = 0; i < nmax && ok; ++i) {
+            const int mv_ = 2 * i + 1, mk_ = 2 * i + 2;
+            bool vw = false, kw = false;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (i >= nt[q] || !ok) continue;
+                ok = mbar_wait_warp(&p_full[q], uint32_t(i & 1));
+                if (ok && !vw) ok = wait_full(mv_);
+                vw = true;
+                if (!ok) continue;
+                tc_fence_after();
+                const uint32_t tV = sKV + (mv_ % NS) * kTile;
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)  // 16 keys a step: 8 columns of P, 16 rows (2048 bytes) of V
+                    umma_bf16_ta_warp(tmem + 256 + HD * q, tmem + 128 * q + 64 + 8 * k, umma_desc(tV + 2048 * k, kHalf, 1024), kIdO,
+                                      uint32_t(i > 0 || k > 0));
+                if (i + 1 == nt[q]) umma_commit_warp(&o_full[q]);
+                if (i + 1 < nt[q]) {
+                    if (!kw) ok = wait_full(mk_);
+                    kw = true;
+                    if (!ok) continue;
+                    tc_fence_after();
+                    qk(q, mk_);
+                }
+            }
+            if (ok) {
+                umma_commit_warp(&empty[mv_ % NS]);
+                if (i + 1 < nmax) umma_commit_warp(&empty[mk_ % NS]);
+            }
+        }
+        umma_commit_warp(drain);  // every MMA issued has completed before the tensor memory is released
+        __syncwarp();
+        mbar_wait_warp(drain, 0);
+    }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode() {
+    static std::once_flag once;
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+        else
+            cudaGetLastError();
+    });
+    return fn;
+}
+
+// Map of one of the cache's tensors: [pages][page rows][kv heads][hd], box 64 elements of one head x up to 128 rows of one
+// page, 128-byte swizzle.
+int cache_map(const vox_cuda_kv_cache &c, const void *base, CUtensorMap &m, const std::string &name) {
+    auto fn = encode();
+    if (!fn) return set_error(VOX_CUDA_ERR_DEVICE, name + ": cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.kv_heads), cuuint64_t(c.page_size), cuuint64_t(c.pages)};
+    // a dimension of one element is never stepped: any stride that the encoder accepts
+    const int64_t page = c.pages > 1 ? c.page_stride : c.row_stride * c.page_size, head = c.kv_heads > 1 ? c.head_stride : c.head_dim;
+    const cuuint64_t strides[3] = {cuuint64_t(head) * 2, cuuint64_t(c.row_stride) * 2, cuuint64_t(page) * 2};
+    const cuuint32_t box[4] = {64, 1, cuuint32_t(c.page_size < kKeys ? c.page_size : kKeys), 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(VOX_CUDA_ERR_ARG, name + ": cache tensor map rejected (code " + std::to_string(int(r)) + ")");
+    return VOX_CUDA_OK;
+}
+
+template <int HD>
+int launch(const AttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int64_t blocks, cudaStream_t st, const char *name) {
+    auto kern = attn_tc_kernel<HD>;
+    // the kernel hands registers between its warpgroups: their sum must be what it was launched with
+    static const int regs = [] {
+        cudaFuncAttributes at = {};
+        return cudaFuncGetAttributes(&at, (const void *)attn_tc_kernel<HD>) == cudaSuccess ? at.numRegs : -1;
+    }();
+    if (regs != kTcRegs) return set_error(VOX_CUDA_ERR_DEVICE, std::string(name) + ": unexpected register count of the tensor-core kernel");
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tc_smem(HD))) != cudaSuccess) return check_launch(name);
+    launch_k(kern, dim3(unsigned(blocks)), kTcThreads, tc_smem(HD), st, a, mk, mv);
+    return check_launch(name);
+}
+
+}  // namespace
+
+int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name) {
+    CUtensorMap mk, mv;
+    int rc = cache_map(c, c.k, mk, name);
+    if (rc == VOX_CUDA_OK) rc = cache_map(c, c.v, mv, name);
+    if (rc != VOX_CUDA_OK) return rc;
+    return c.head_dim == 64 ? launch<64>(a, mk, mv, blocks, st, name) : launch<128>(a, mk, mv, blocks, st, name);
+}
+
+int attn_tc_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+
+}  // namespace voxcuda

@@ -1,5 +1,5 @@
 // Attention over a paged key/value cache: vox_cuda_attn_paged and vox_cuda_attn_prefix, their split of the work, the
-// CUDA-core kernel (every type, exact to f32) and the join of split rows.
+// CUDA-core kernel (f32 caches) and the join of split rows.
 #include <cmath>
 
 #include "attn.cuh"
@@ -28,8 +28,9 @@ __device__ __forceinline__ float load_f(const __nv_bfloat16 *p) { return __bfloa
 // loop over the keys has no exchange between groups: per key and row one dot product (a butterfly over the LPK lanes),
 // one 2^x, and one multiply-add per element of v. Every warp takes each kVecWarps-th run of KPI keys, U loads of K and U
 // of V in flight before the first is used. Groups and warps are joined once, at the end.
-template <typename QT, typename CT, int HD, int R>
+template <typename QT, int HD, int R>
 __global__ void __launch_bounds__(kVecThreads) attn_vec_kernel(const AttnArgs a) {
+    using CT = float;
     constexpr int V = 16 / int(sizeof(CT));     // elements a lane holds of a key
     constexpr int LPK = HD / V, KPW = 32 / LPK; // lanes a key, keys a warp load
     constexpr int U = R <= 2 ? 8 : 4;           // loads of K (and of V) in flight
@@ -213,7 +214,7 @@ int ceil_div(int64_t x, int64_t y) { return int((x + y - 1) / y); }
 
 // How a call is cut: which kernels take its parts, rows a block, row tiles, key splits.
 struct AttnShape {
-    bool own_tc, pre_tc, concat;
+    bool own_tc, pre_tc, concat, mma;  // mma: the rest goes to attn_mma.cu, else to the CUDA cores
     int rows_blk, tc_rows;
     int own_tiles, own_splits, own_chunk;
     int pre_tiles, pre_splits, pre_chunk;
@@ -229,10 +230,11 @@ void cut_keys(int64_t keys, int64_t want, int &splits, int &chunk) {
     chunk = int(per * 128);
 }
 
-AttnShape attn_shape(const PagedArgs &p, int64_t max_q, int64_t max_kv, int64_t prefix_len, bool tc_types) {
+AttnShape attn_shape(const PagedArgs &p, int64_t max_q, int64_t max_kv, int64_t prefix_len, bool tc_types, bool mma, bool f32) {
     AttnShape s = {};
     const int64_t rows = max_q * p.group, all = int64_t(p.tokens) * p.group, sms = sm_count();
-    s.rows_blk = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    s.mma = mma;
+    s.rows_blk = mma ? (rows <= 8 || f32 ? 8 : 16) : rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
     s.own_tc = tc_types && rows > 16;
     s.pre_tc = tc_types && all > 16;
     s.concat = prefix_len > 0 && s.own_tc && rows >= 64;
@@ -267,12 +269,12 @@ size_t workspace_of(const PagedArgs &p, const AttnShape &s, int head_dim) {
     return slots * size_t(head_dim) * sizeof(float) + slots * sizeof(float2);
 }
 
-template <typename QT, typename CT, int HD>
+template <typename QT, int HD>
 int launch_vec(const AttnArgs &a, const AttnShape &s, int64_t blocks, cudaStream_t st, const char *name) {
-    auto kern = s.rows_blk == 1   ? attn_vec_kernel<QT, CT, HD, 1>
-                : s.rows_blk == 2 ? attn_vec_kernel<QT, CT, HD, 2>
-                : s.rows_blk == 4 ? attn_vec_kernel<QT, CT, HD, 4>
-                                  : attn_vec_kernel<QT, CT, HD, 8>;
+    auto kern = s.rows_blk == 1   ? attn_vec_kernel<QT, HD, 1>
+                : s.rows_blk == 2 ? attn_vec_kernel<QT, HD, 2>
+                : s.rows_blk == 4 ? attn_vec_kernel<QT, HD, 4>
+                                  : attn_vec_kernel<QT, HD, 8>;
     launch_k(kern, dim3(unsigned(blocks)), kVecThreads, 0, st, a);
     return check_launch(name);
 }
@@ -299,7 +301,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     const int64_t max_q = batch->q_start == nullptr ? a.p.q_per : batch->max_q > 0 && batch->max_q < batch->tokens ? batch->max_q : batch->tokens;
     const int64_t max_kv = batch->max_kv > 0 && batch->max_kv < a.p.cap ? batch->max_kv : a.p.cap;
     const bool tc_types = dtype == VOX_CUDA_BF16 && cache->dtype == VOX_CUDA_BF16;
-    const AttnShape s = attn_shape(a.p, max_q, max_kv, prefix_len, tc_types);
+    const AttnShape s = attn_shape(a.p, max_q, max_kv, prefix_len, tc_types, cache->dtype == VOX_CUDA_BF16, dtype == VOX_CUDA_F32);
     VOX_REQUIRE(s.own_blocks + s.pre_blocks < (int64_t(1) << 31), nm + ": sizes out of range");
     const size_t need = workspace_of(a.p, s, hd);
     if (want) {
@@ -331,7 +333,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + slots * size_t(hd) * sizeof(float));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     using bf = __nv_bfloat16;
-    const bool qf = dtype == VOX_CUDA_F32, cf = cache->dtype == VOX_CUDA_F32;
+    const bool qf = dtype == VOX_CUDA_F32;
     int r = VOX_CUDA_OK;
     if (s.pre_blocks > 0 && s.pre_tc) {
         a.tc_prefix = 1;
@@ -344,12 +346,12 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     } else {
         a.pre_blocks = s.pre_tc ? 0 : int32_t(s.pre_blocks);
         const int64_t n = a.pre_blocks + s.own_blocks;
-        if (hd == 64)
-            r = qf ? (cf ? launch_vec<float, float, 64>(a, s, n, st, name) : launch_vec<float, bf, 64>(a, s, n, st, name))
-                   : (cf ? launch_vec<bf, float, 64>(a, s, n, st, name) : launch_vec<bf, bf, 64>(a, s, n, st, name));
+        if (s.mma)
+            r = attn_mma_launch(a, hd, s.rows_blk, dtype, n, st, name);
+        else if (hd == 64)
+            r = qf ? launch_vec<float, 64>(a, s, n, st, name) : launch_vec<bf, 64>(a, s, n, st, name);
         else
-            r = qf ? (cf ? launch_vec<float, float, 128>(a, s, n, st, name) : launch_vec<float, bf, 128>(a, s, n, st, name))
-                   : (cf ? launch_vec<bf, float, 128>(a, s, n, st, name) : launch_vec<bf, bf, 128>(a, s, n, st, name));
+            r = qf ? launch_vec<float, 128>(a, s, n, st, name) : launch_vec<bf, 128>(a, s, n, st, name);
     }
     if (r != VOX_CUDA_OK || a.splits == 1) return r;
     if (hd == 64) return qf ? launch_merge<float, 64>(a, st, name) : launch_merge<bf, 64>(a, st, name);

@@ -88,6 +88,8 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
 }
 
 
+// Few rows on a bf16 cache (attn_mma.cu): rows_blk 8, or 16 (bf16 activations).
+int attn_mma_launch(const AttnArgs &a, int head_dim, int rows_blk, int dtype, int64_t blocks, cudaStream_t st, const char *name);
 // The tensor-core path (attn_tc.cu).
 int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name);
 

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -517,10 +518,10 @@ class _KvCache(ctypes.Structure):
                [(n, ctypes.c_int64) for n in ("page_stride", "row_stride", "head_stride")]
 
 
-class _KvBatch(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("page_table", "kv_len", "q_start")] + \
-               [(n, ctypes.c_int64) for n in ("table_stride", "tokens")] + \
-               [(n, ctypes.c_int32) for n in ("seqs", "table_width", "max_q", "max_kv")]
+# vox_cuda_kv_batch: page_table, kv_len, q_start; table_stride, tokens; seqs, table_width, max_q, max_kv
+_pack_batch = struct.Struct("@3P2q4i").pack
+_ACT = {torch.float32: F32, torch.bfloat16: BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without building a Stream object
 
 
 class PagedKV:
@@ -549,41 +550,67 @@ class PagedKV:
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
         self._c = _KvCache(k.data_ptr(), v.data_ptr(), F32 if k.dtype == torch.float32 else BF16, self.page_size, self.pages,
                            self.kv_heads, self.head_dim, *k.stride()[:3])
-        self._cp = ctypes.byref(self._c)
+        self._cp, self._dev = ctypes.byref(self._c), k.get_device()
         self._need = {}  # workspace bytes by batch shape
-
-    def _ints(self, t, name, dims):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.k.device or t.dim() != dims or \
-                (t.shape[-1] > 1 and t.stride(-1) != 1):
-            raise VoxCudaError(-6, f"{name} must be an int32 tensor of {dims} dimension(s) on the cache's device, its last one contiguous")
-        return t.data_ptr()
+        self._c_append, self._c_attend, self._c_prefix = lib.vox_cuda_kv_append, lib.vox_cuda_attn_paged, lib.vox_cuda_attn_prefix
 
     def _batch(self, tokens, page_table, kv_len, q_start, max_q, max_kv):
-        pt, pl = self._ints(page_table, "page_table", 2), self._ints(kv_len, "kv_len", 1)
-        ps = None if q_start is None else self._ints(q_start, "q_start", 1)
+        """The packed vox_cuda_kv_batch of a call."""
+        dev, i32 = self._dev, torch.int32
+        if not (isinstance(page_table, torch.Tensor) and page_table.dtype is i32 and page_table.get_device() == dev and page_table.dim() == 2):
+            raise VoxCudaError(-6, "page_table must be an int32 tensor [seqs][width] on the cache's device")
+        if not (isinstance(kv_len, torch.Tensor) and kv_len.dtype is i32 and kv_len.get_device() == dev and kv_len.dim() == 1 and
+                kv_len.is_contiguous()):
+            raise VoxCudaError(-6, "kv_len must be a contiguous int32 tensor [seqs] on the cache's device")
         seqs, width = page_table.shape
-        if kv_len.shape[0] != seqs or (q_start is not None and q_start.shape[0] != seqs + 1):
+        stride = page_table.stride()
+        if seqs <= 1:
+            stride = (width, stride[1])
+        if (width > 1 and stride[1] != 1) or stride[0] < width:
+            raise VoxCudaError(-6, "page_table's rows must be contiguous and not overlap")
+        start = 0
+        if q_start is not None:
+            if not (isinstance(q_start, torch.Tensor) and q_start.dtype is i32 and q_start.get_device() == dev and q_start.is_contiguous() and
+                    q_start.dim() == 1):
+                raise VoxCudaError(-6, "q_start must be a contiguous int32 tensor [seqs + 1] on the cache's device")
+            start = q_start.data_ptr()
+            if q_start.numel() != seqs + 1:
+                raise VoxCudaError(-6, "page_table [seqs][width], kv_len [seqs] and q_start [seqs + 1] must agree")
+        if kv_len.numel() != seqs:
             raise VoxCudaError(-6, "page_table [seqs][width], kv_len [seqs] and q_start [seqs + 1] must agree")
-        return _KvBatch(pt, pl, ps, page_table.stride(0) if seqs > 1 else width, tokens, seqs, width, max_q, max_kv)
+        return _pack_batch(page_table.data_ptr(), kv_len.data_ptr(), start, stride[0], tokens, seqs, width, max_q, max_kv)
 
     def _rows(self, t, name, width):
-        """(dtype, tokens, row stride) of activations [tokens][...] whose trailing dimensions are contiguous."""
-        if not isinstance(t, torch.Tensor) or t.device != self.k.device:
+        """(dtype, tokens, row stride, elements a token) of activations [tokens][...] contiguous within a token."""
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._dev:
             raise VoxCudaError(-6, f"{name} must be a tensor on the cache's device (vox_b200 has no CPU path)")
-        if t.dim() == 3:
-            ok, inner = t.stride(2) == 1 and (t.stride(1) == t.shape[2] or t.shape[1] == 1), t.shape[1] * t.shape[2]
+        dt = _ACT.get(t.dtype)
+        if dt is None:
+            raise VoxCudaError(-6, f"{name} must be float32 or bfloat16, got {t.dtype}")
+        shape = t.shape
+        if len(shape) == 2:
+            tokens, inner = shape
+        elif len(shape) == 3:
+            tokens, inner = shape[0], shape[1] * shape[2]
         else:
-            ok, inner = t.dim() == 2 and t.stride(1) == 1, t.shape[-1]
-        if not ok or (width and inner != width):
+            tokens, inner = 0, -1
+        if t.is_contiguous():
+            stride, ok = inner, True
+        else:
+            st = t.stride()
+            stride, ok = st[0] if tokens > 1 else inner, st[-1] == 1 and (len(st) == 2 or st[1] == shape[2] or shape[1] == 1)
+        if not ok or inner < 0 or (width and inner != width):
             raise VoxCudaError(-6, f"{name} must be [tokens][heads * head_dim] or [tokens][heads][head_dim], contiguous within a token"
                                + (f", {width} elements each" if width else ""))
-        if t.dtype == torch.float32:
-            dt = F32
-        elif t.dtype == torch.bfloat16:
-            dt = BF16
-        else:
-            raise VoxCudaError(-6, f"{name} must be float32 or bfloat16, got {t.dtype}")
-        return dt, t.shape[0], t.stride(0) if t.shape[0] > 1 else inner, inner
+        return dt, tokens, stride, inner
+
+    def _vec(self, t, name):
+        """Pointer of a contiguous f32 parameter, or None."""
+        if t is None:
+            return None
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._dev or t.dtype is not torch.float32 or not t.is_contiguous():
+            raise VoxCudaError(-6, f"{name} must be a contiguous float32 tensor on the cache's device")
+        return t.data_ptr()
 
     def append(self, qkv, cs, page_table, kv_len, heads: int, q_start=None, q_norm_w=None, k_norm_w=None, eps: float = 1e-6,
                q=None) -> torch.Tensor:
@@ -592,19 +619,21 @@ class PagedKV:
         [tokens][heads * head_dim] (qkv's dtype). cs: rope_table(inv_freq, 0, n) of all positions in use."""
         hd = self.head_dim
         dt, tokens, stride, _ = self._rows(qkv, "qkv", (heads + 2 * self.kv_heads) * hd)
-        if _f32(cs, "cs") and (cs.dim() != 3 or cs.shape[1] != hd // 2 or cs.shape[2] != 2):
+        csp, qnp, knp = self._vec(cs, "cs"), self._vec(q_norm_w, "q_norm_w"), self._vec(k_norm_w, "k_norm_w")
+        if cs is None or cs.dim() != 3 or cs.numel() != cs.shape[0] * hd or cs.shape[2] != 2:
             raise VoxCudaError(-6, "cs must be [positions][head_dim / 2][2]")
-        for w, nm in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-            if w is not None and w.numel() != hd:
-                raise VoxCudaError(-6, f"{nm} must have head_dim elements")
+        if (qnp is not None and q_norm_w.numel() != hd) or (knp is not None and k_norm_w.numel() != hd):
+            raise VoxCudaError(-6, "q_norm_w and k_norm_w must have head_dim elements")
         if q is None:
-            q = torch.empty((tokens, heads * hd), dtype=qkv.dtype, device=qkv.device)
-        qdt, qtok, qstride, _ = self._rows(q, "q", heads * hd)
-        if qdt != dt or qtok != tokens:
-            raise VoxCudaError(-6, "q must have qkv's dtype and tokens")
-        b = self._batch(tokens, page_table, kv_len, q_start, 0, 0)
-        _check(lib.vox_cuda_kv_append(self._cp, ctypes.byref(b), qkv.data_ptr(), stride, _f32(q_norm_w, "q_norm_w"),
-                                      _f32(k_norm_w, "k_norm_w"), cs.data_ptr(), cs.shape[0], q.data_ptr(), qstride, heads, eps, dt, _stream(qkv)))
+            q, qstride = qkv.new_empty((tokens, heads * hd)), heads * hd
+        else:
+            qdt, qtok, qstride, _ = self._rows(q, "q", heads * hd)
+            if qdt != dt or qtok != tokens:
+                raise VoxCudaError(-6, "q must have qkv's dtype and tokens")
+        rc = self._c_append(self._cp, self._batch(tokens, page_table, kv_len, q_start, 0, 0), qkv.data_ptr(), stride, qnp, knp, csp,
+                                    cs.shape[0], q.data_ptr(), qstride, heads, eps, dt, _raw_stream(self._dev))
+        if rc:
+            _check(rc)
         return q
 
     def attend(self, q, page_table, kv_len, q_start=None, max_q: int = 0, max_kv: int = 0, scale: float | None = None,
@@ -618,7 +647,9 @@ class PagedKV:
                       scale: float | None = None, out=None) -> torch.Tensor:
         """attend() for sequences that all stand behind one shared prefix: every token sees the prefix_len rows behind
         prefix_pages (int32), read once for the whole batch, and then its own sequence's rows as in attend()."""
-        self._ints(prefix_pages, "prefix_pages", 1)
+        if not (isinstance(prefix_pages, torch.Tensor) and prefix_pages.dtype is torch.int32 and prefix_pages.get_device() == self._dev and
+                prefix_pages.dim() == 1 and prefix_pages.is_contiguous()):
+            raise VoxCudaError(-6, "prefix_pages must be a contiguous int32 tensor on the cache's device")
         if not 0 <= prefix_len <= prefix_pages.shape[0] * self.page_size:
             raise VoxCudaError(-6, "prefix_len must fit prefix_pages")
         return self._attend(q, prefix_pages, prefix_len, page_table, kv_len, q_start, max_q, max_kv, scale, 0, out)
@@ -630,31 +661,34 @@ class PagedKV:
         if heads * hd != inner or (q.dim() == 3 and q.shape[2] != hd):
             raise VoxCudaError(-6, "q must hold whole heads of the cache's head_dim")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        odt, otok, ostride, _ = self._rows(out, "out", inner)
-        if odt != dt or otok != tokens:
-            raise VoxCudaError(-6, "out must have q's dtype and tokens")
+            out, ostride = q.new_empty(q.shape), inner
+        else:
+            odt, otok, ostride, _ = self._rows(out, "out", inner)
+            if odt != dt or otok != tokens:
+                raise VoxCudaError(-6, "out must have q's dtype and tokens")
         b = self._batch(tokens, page_table, kv_len, q_start, max_q, max_kv)
-        bp = ctypes.byref(b)
-        key = (b.seqs, tokens, b.table_width, max_q, max_kv, q_start is None, prefix_len, heads, window, dt)
+        # the bytes are a function of the batch's shape alone
+        key = (page_table.shape, tokens, max_q, max_kv, q_start is None, prefix_len, heads, window, dt)
         need = self._need.get(key)
         if need is None:
             n = ctypes.c_size_t()
-            _check(lib.vox_cuda_attn_workspace(self._cp, bp, prefix_len, heads, window, dt, ctypes.byref(n)))
+            _check(lib.vox_cuda_attn_workspace(self._cp, b, prefix_len, heads, window, dt, ctypes.byref(n)))
             if len(self._need) > 4096:
                 self._need.clear()
             need = self._need[key] = n.value
         # scratch of this call alone, from torch's allocator: it is reused only behind this call on the same stream
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        wp = None if ws is None else ws.data_ptr()
         if scale is None:
             scale = hd ** -0.5
         if prefix_pages is None:
-            rc = lib.vox_cuda_attn_paged(self._cp, bp, q.data_ptr(), stride, out.data_ptr(), ostride, heads, scale, window, dt,
-                                         None if ws is None else ws.data_ptr(), need, _stream(q))
+            rc = self._c_attend(self._cp, b, q.data_ptr(), stride, out.data_ptr(), ostride, heads, scale, window, dt, wp, need,
+                                         _raw_stream(self._dev))
         else:
-            rc = lib.vox_cuda_attn_prefix(self._cp, bp, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), stride, out.data_ptr(), ostride,
-                                          heads, scale, dt, None if ws is None else ws.data_ptr(), need, _stream(q))
-        _check(rc)
+            rc = self._c_prefix(self._cp, b, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), stride, out.data_ptr(), ostride,
+                                          heads, scale, dt, wp, need, _raw_stream(self._dev))
+        if rc:
+            _check(rc)
         return out
 
 

@@ -2,47 +2,33 @@
 // CUDA-core kernel (f32 caches) and the join of split rows.
 #include <cmath>
 
-#include "attn.cuh"
-#include "sfu.cuh"
+#include "attn_rows.cuh"
 
 namespace voxcuda {
 namespace {
 
-constexpr int kVecThreads = 128;
-constexpr int kVecWarps = kVecThreads / 32;
-
-template <typename T> struct DtOf;
-template <> struct DtOf<float> { static constexpr int v = VOX_CUDA_F32; };
-template <> struct DtOf<__nv_bfloat16> { static constexpr int v = VOX_CUDA_BF16; };
-
-__device__ __forceinline__ void store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
-    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-}
 __device__ __forceinline__ float load_f(const float *p) { return *p; }
 __device__ __forceinline__ float load_f(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 
-// softmax(scale q k^T) v on the CUDA cores, f32 throughout: R rows (query heads that share a key/value head, of one or
-// more tokens) against the keys of one split. Lane layout: a key's row of HD elements takes LPK lanes of 16 bytes, so a
-// warp load brings KPW keys; each group of LPK lanes keeps its own running maximum, sum and output of every row, so the
-// loop over the keys has no exchange between groups: per key and row one dot product (a butterfly over the LPK lanes),
-// one 2^x, and one multiply-add per element of v. Every warp takes each kVecWarps-th run of KPI keys, U loads of K and U
-// of V in flight before the first is used. Groups and warps are joined once, at the end.
-template <typename QT, int HD, int R>
-__global__ void __launch_bounds__(kVecThreads) attn_vec_kernel(const AttnArgs a) {
-    using CT = float;
-    constexpr int V = 16 / int(sizeof(CT));     // elements a lane holds of a key
-    constexpr int LPK = HD / V, KPW = 32 / LPK; // lanes a key, keys a warp load
-    constexpr int U = R <= 2 ? 8 : 4;           // loads of K (and of V) in flight
-    constexpr int KPI = KPW * U;                // keys a step; divides or is a multiple of 16
-    __shared__ float s_acc[kVecWarps][R][HD];
-    __shared__ float2 s_ml[kVecWarps][R];
-    pdl_enter();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane / LPK, e0 = (lane % LPK) * V;
-    const AttnJob j = attn_job(a, blockIdx.x);
-    const CT *K = static_cast<const CT *>(a.p.k) + int64_t(j.kvh) * a.p.head_stride + e0;
-    const CT *Vp = static_cast<const CT *>(a.p.v) + int64_t(j.kvh) * a.p.head_stride + e0;
-    for (int row0 = j.tile * R; row0 < j.rows; row0 += j.tiles * R) {
+// softmax(scale q k^T) v on the CUDA cores for an f32 cache, f32 throughout: R rows (query heads that share a key/value
+// head, of one or more tokens) against a range of keys. Lane layout: a key's row of HD elements takes LPK lanes of 16
+// bytes, so a warp load brings KPW keys; each group of LPK lanes keeps its own running maximum, sum and output of every
+// row, so the loop over the keys has no exchange between groups: per key and row one dot product (a butterfly over the LPK
+// lanes), one 2^x, and one multiply-add per element of v. Every warp takes each kRowsWarps-th run of KPI keys, U loads of K
+// and U of V in flight before the first is used. The groups of a warp are joined at the end.
+template <typename QT, int HD_, int R>
+struct VecCore {
+    using Q = QT;
+    static constexpr int HD = HD_, RB = R, kMinBlocks = R <= 4 ? 4 : 2;
+
+    static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB]) {
+        constexpr int V = 4;                        // elements a lane holds of a key
+        constexpr int LPK = HD / V, KPW = 32 / LPK; // lanes a key, keys a warp load
+        constexpr int U = R <= 2 ? 8 : 4;           // loads of K (and of V) in flight
+        constexpr int KPI = KPW * U;                // keys a step; divides or is a multiple of 16
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane / LPK, e0 = (lane % LPK) * V, row0 = j.row0;
+        const float *K = static_cast<const float *>(a.p.k) + int64_t(j.kvh) * a.p.head_stride + e0;
+        const float *Vp = static_cast<const float *>(a.p.v) + int64_t(j.kvh) * a.p.head_stride + e0;
         float2 q[R][V / 2], acc[R][V / 2];
         float m[R], l[R];
         int hi[R], lo[R];
@@ -62,7 +48,7 @@ __global__ void __launch_bounds__(kVecThreads) attn_vec_kernel(const AttnArgs a)
             lo[r] = a.window > 0 && j.causal ? max(j.base + i + 1 - a.window, j.k0) : j.k0;
             kmin = min(kmin, lo[r]), kend = max(kend, hi[r]);
         }
-        for (int base = (kmin & ~15) + warp * KPI; base < kend; base += kVecWarps * KPI) {
+        for (int base = (kmin & ~15) + warp * KPI; base < kend; base += kRowsWarps * KPI) {
             uint4 kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -79,7 +65,7 @@ __global__ void __launch_bounds__(kVecThreads) attn_vec_kernel(const AttnArgs a)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float2 kf[V / 2];
-                unpack2<DtOf<CT>::v>(kr[u], kf);
+                unpack2<VOX_CUDA_F32>(kr[u], kf);
                 const int key = base + u * KPW + grp;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -112,7 +98,7 @@ __global__ void __launch_bounds__(kVecThreads) attn_vec_kernel(const AttnArgs a)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float2 vf[V / 2];
-                unpack2<DtOf<CT>::v>(vr[u], vf);
+                unpack2<VOX_CUDA_F32>(vr[u], vf);
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -141,36 +127,18 @@ __global__ void __launch_bounds__(kVecThreads) attn_vec_kernel(const AttnArgs a)
                 if (lane == 0) s_ml[warp][r] = make_float2(m[r], l[r]);
             }
         }
-        __syncthreads();
-        for (int x = threadIdx.x; x < R * (HD / 4); x += kVecThreads) {
-            const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
-            if (row0 + r >= j.rows) break;
-            float mx = -INFINITY, lt = 0.f;
-#pragma unroll
-            for (int w = 0; w < kVecWarps; ++w) mx = fmaxf(mx, s_ml[w][r].x);
-            const float ms = mx == -INFINITY ? 0.f : mx;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kVecWarps; ++w) {
-                const float wt = ex2_approx(s_ml[w][r].x - ms);
-                const float4 t = *reinterpret_cast<const float4 *>(&s_acc[w][r][d]);
-                lt = fmaf(s_ml[w][r].y, wt, lt);
-                o.x = fmaf(t.x, wt, o.x), o.y = fmaf(t.y, wt, o.y), o.z = fmaf(t.z, wt, o.z), o.w = fmaf(t.w, wt, o.w);
-            }
-            const int i = int(a.gdiv.div(uint32_t(row0 + r))), h = j.kvh * a.p.group + row0 + r - i * a.p.group;
-            const int tok = j.tok0 + i;
-            if (a.splits == 1) {
-                const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // a row that sees no key gives zeros
-                store4(static_cast<QT *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d,
-                       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-            } else {
-                const int64_t slot = (int64_t(tok) * a.p.heads + h) * a.splits + j.split;
-                store4(a.part_o + slot * HD + d, o);
-                if (d == 0) a.part_ml[slot] = make_float2(mx, lt);
-            }
-        }
-        __syncthreads();
     }
+};
+
+template <typename QT, typename F>
+int with_vec(int head_dim, int rows_blk, F f) {
+    if (head_dim == 64)
+        return rows_blk == 1 ? f(VecCore<QT, 64, 1>()) : rows_blk == 2 ? f(VecCore<QT, 64, 2>()) : rows_blk == 4 ? f(VecCore<QT, 64, 4>()) : f(VecCore<QT, 64, 8>());
+    return rows_blk == 1 ? f(VecCore<QT, 128, 1>()) : rows_blk == 2 ? f(VecCore<QT, 128, 2>()) : rows_blk == 4 ? f(VecCore<QT, 128, 4>()) : f(VecCore<QT, 128, 8>());
+}
+template <typename F>
+int with_vec(int dtype, int head_dim, int rows_blk, F f) {
+    return dtype == VOX_CUDA_F32 ? with_vec<float>(head_dim, rows_blk, f) : with_vec<__nv_bfloat16>(head_dim, rows_blk, f);
 }
 
 // Joins the splits of each row: one warp a row, lanes over the splits for the weights, then over the head's elements.
@@ -214,11 +182,14 @@ int ceil_div(int64_t x, int64_t y) { return int((x + y - 1) / y); }
 
 // How a call is cut: which kernels take its parts, rows a block, row tiles, key splits.
 struct AttnShape {
-    bool own_tc, pre_tc, concat, mma;  // mma: the rest goes to attn_mma.cu, else to the CUDA cores
+    bool own_tc, pre_tc, concat, mma;  // mma: what the tensor-core kernel does not take goes to attn_mma.cu, else to the CUDA cores
+    int frame;                         // of the own keys, where the tensor-core kernel does not take them
     int rows_blk, tc_rows;
     int own_tiles, own_splits, own_chunk;
     int pre_tiles, pre_splits, pre_chunk;
-    int64_t own_blocks, pre_blocks;
+    int cluster, stream_keys, stream_rows;
+    int64_t own_units, pre_blocks;     // blocks, or clusters
+    int slots;                         // of a row in the workspace
 };
 
 // Keys cut into at most `want` splits of whole 128-key tiles.
@@ -230,53 +201,77 @@ void cut_keys(int64_t keys, int64_t want, int &splits, int &chunk) {
     chunk = int(per * 128);
 }
 
-AttnShape attn_shape(const PagedArgs &p, int64_t max_q, int64_t max_kv, int64_t prefix_len, bool tc_types, bool mma, bool f32) {
+AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cache, int64_t max_q, int64_t max_kv, int64_t prefix_len) {
     AttnShape s = {};
-    const int64_t rows = max_q * p.group, all = int64_t(p.tokens) * p.group, sms = sm_count();
-    s.mma = mma;
-    s.rows_blk = mma ? (rows <= 8 || f32 ? 8 : 16) : rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    const int64_t rows = max_q * p.group, all = int64_t(p.tokens) * p.group, sms = sm_count(), base = int64_t(p.seqs) * p.kv_heads;
+    const bool f32 = dtype == VOX_CUDA_F32, tc_types = !f32 && bf16_cache;
+    s.mma = bf16_cache;
+    s.rows_blk = s.mma ? (rows <= 8 || f32 ? 8 : 16) : rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
     s.own_tc = tc_types && rows > 16;
     s.pre_tc = tc_types && all > 16;
     s.concat = prefix_len > 0 && s.own_tc && rows >= 64;
-    if (s.own_tc) {
-        // row tiles of all sequences together: exact for equal counts, else one more a sequence at most
-        auto tiles = [&](int64_t rb) { return p.q_start ? all / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
-        s.tc_rows = tiles(256) * p.kv_heads >= sms / 2 ? 256 : 128;
-        s.own_tiles = int(tiles(s.tc_rows));
-        const int64_t own = int64_t(s.own_tiles) * p.kv_heads;
-        cut_keys(max_kv, s.concat ? 1 : own < sms ? sms / own : 1, s.own_splits, s.own_chunk);
-        s.own_blocks = own * s.own_splits;
-    } else {
-        s.own_tiles = ceil_div(rows > 0 ? rows : 1, s.rows_blk);
-        const int64_t own = int64_t(p.seqs) * p.kv_heads * s.own_tiles;
-        cut_keys(max_kv, ceil_div(sms * 4, own), s.own_splits, s.own_chunk);
-        s.own_blocks = own * s.own_splits;
-    }
     if (prefix_len > 0 && !s.concat) {
-        if (s.pre_tc) s.tc_rows = all > 128 ? 256 : 128;
-        s.pre_tiles = ceil_div(all, s.pre_tc ? s.tc_rows : s.rows_blk);
+        const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.rows_blk;
+        if (s.pre_tc) s.tc_rows = rb;
+        s.pre_tiles = ceil_div(all, rb);
         const int64_t pre = int64_t(p.kv_heads) * s.pre_tiles;
         cut_keys(prefix_len, s.pre_tc ? (pre < sms ? sms / pre : 1) : ceil_div(sms * 4, pre), s.pre_splits, s.pre_chunk);
         s.pre_blocks = pre * s.pre_splits;
     }
+    if (s.own_tc) {
+        // row tiles of all sequences together: exact for equal counts, else one more a sequence at most
+        auto tiles = [&](int64_t rb) { return p.q_start ? all / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
+        if (s.tc_rows == 0) s.tc_rows = tiles(256) * p.kv_heads >= sms / 2 ? 256 : 128;
+        s.own_tiles = int(tiles(s.tc_rows));
+        const int64_t own = int64_t(s.own_tiles) * p.kv_heads;
+        cut_keys(max_kv, s.concat ? 1 : own < sms ? sms / own : 1, s.own_splits, s.own_chunk);
+        s.own_units = own * s.own_splits;
+    } else if (rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc)) {
+        // one row tile a sequence: a cluster for each sequence and key/value head where one wave of blocks holds them all
+        // with at most 512 keys each, else equal runs of all sequences' tiles
+        const int64_t resident = s.mma ? attn_mma_resident(head_dim, s.rows_blk, dtype)
+                                       : with_vec(dtype, head_dim, s.rows_blk, [](auto core) {
+                                             return resident_blocks((const void *)attn_stream_kernel<decltype(core)>, kRowsThreads, 0);
+                                         });
+        int c = 8;
+        while (c > 1 && (base * c > resident || 32 * c > max_kv)) c /= 2;
+        if (base * c <= resident && max_kv <= 512 * c) {
+            s.frame = kFrameCluster;
+            s.cluster = c;
+            s.own_units = base;
+        } else {
+            s.frame = kFrameStream;
+            s.stream_keys = head_dim == 64 ? 128 : 64;
+            s.stream_rows = int(p.q_start ? s.rows_blk : rows);
+            const int64_t tiles = base * ((max_kv + s.stream_keys - 1) / s.stream_keys);
+            s.own_units = tiles < 1 ? 1 : tiles < resident ? tiles : resident;
+        }
+    } else {
+        s.own_tiles = ceil_div(rows > 0 ? rows : 1, s.rows_blk);
+        const int64_t own = base * s.own_tiles;
+        cut_keys(max_kv, ceil_div(sms * 4, own), s.own_splits, s.own_chunk);
+        s.own_units = own * s.own_splits;
+    }
+    s.slots = s.pre_splits + s.own_splits;
     return s;
 }
 
-size_t workspace_of(const PagedArgs &p, const AttnShape &s, int head_dim) {
-    const int64_t splits = s.own_splits + s.pre_splits;
-    if (splits <= 1) return 0;
-    const size_t slots = size_t(p.tokens) * size_t(p.heads) * size_t(splits);
-    return slots * size_t(head_dim) * sizeof(float) + slots * sizeof(float2);
-}
-
-template <typename QT, int HD>
-int launch_vec(const AttnArgs &a, const AttnShape &s, int64_t blocks, cudaStream_t st, const char *name) {
-    auto kern = s.rows_blk == 1   ? attn_vec_kernel<QT, HD, 1>
-                : s.rows_blk == 2 ? attn_vec_kernel<QT, HD, 2>
-                : s.rows_blk == 4 ? attn_vec_kernel<QT, HD, 4>
-                                  : attn_vec_kernel<QT, HD, 8>;
-    launch_k(kern, dim3(unsigned(blocks)), kVecThreads, 0, st, a);
-    return check_launch(name);
+// The workspace: the slots of every row (where a row has more than one, or its own keys are taken by another frame), then
+// the parts of the stream frame. Offsets in bytes; returns the size.
+struct Scratch {
+    size_t part_ml, stream_o, stream_ml, bytes;
+    bool partial;
+};
+Scratch scratch_of(const PagedArgs &p, const AttnShape &s, int head_dim) {
+    Scratch w = {};
+    w.partial = s.slots > 1 || (s.pre_splits > 0 && s.own_splits == 0);
+    const size_t slots = w.partial ? size_t(p.tokens) * size_t(p.heads) * size_t(s.slots) : 0;
+    const size_t parts = s.own_splits == 0 && s.frame == kFrameStream ? size_t(s.own_units) * 2 * size_t(s.rows_blk) : 0;
+    w.part_ml = slots * size_t(head_dim) * sizeof(float);
+    w.stream_o = (w.part_ml + slots * sizeof(float2) + 255) & ~size_t(255);
+    w.stream_ml = w.stream_o + parts * size_t(head_dim) * sizeof(float);
+    w.bytes = w.stream_ml + parts * sizeof(float2);
+    return w;
 }
 
 template <typename QT, int HD>
@@ -289,32 +284,33 @@ int launch_merge(const AttnArgs &a, cudaStream_t st, const char *name) {
 int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, const int32_t *prefix_pages, int64_t prefix_len, const void *q,
              int64_t q_stride, void *out, int64_t out_stride, int64_t heads, float scale, int64_t window, int dtype, void *workspace,
              size_t workspace_bytes, size_t *want, void *stream, const char *name) {
-    const std::string nm(name);
     AttnArgs a = {};
     const int rc = paged_args(cache, batch, heads, name, a.p);
     if (rc != VOX_CUDA_OK) return rc;
-    VOX_REQUIRE(is_act_dtype(dtype), nm + ": dtype must be f32 or bf16");
-    VOX_REQUIRE(window >= 0 && prefix_len >= 0 && prefix_len < (int64_t(1) << 30), nm + ": window or prefix_len out of range");
+    VOX_REQUIRE(is_act_dtype(dtype), std::string(name) + ": dtype must be f32 or bf16");
+    VOX_REQUIRE(window >= 0 && prefix_len >= 0 && prefix_len < (int64_t(1) << 30), std::string(name) + ": window or prefix_len out of range");
     if (want) *want = 0;
     if (batch->seqs == 0 || batch->tokens == 0) return VOX_CUDA_OK;
     const int hd = cache->head_dim;
     const int64_t max_q = batch->q_start == nullptr ? a.p.q_per : batch->max_q > 0 && batch->max_q < batch->tokens ? batch->max_q : batch->tokens;
     const int64_t max_kv = batch->max_kv > 0 && batch->max_kv < a.p.cap ? batch->max_kv : a.p.cap;
-    const bool tc_types = dtype == VOX_CUDA_BF16 && cache->dtype == VOX_CUDA_BF16;
-    const AttnShape s = attn_shape(a.p, max_q, max_kv, prefix_len, tc_types, cache->dtype == VOX_CUDA_BF16, dtype == VOX_CUDA_F32);
-    VOX_REQUIRE(s.own_blocks + s.pre_blocks < (int64_t(1) << 31), nm + ": sizes out of range");
-    const size_t need = workspace_of(a.p, s, hd);
+    const AttnShape s = attn_shape(a.p, hd, dtype, cache->dtype == VOX_CUDA_BF16, max_q, max_kv, prefix_len);
+    VOX_REQUIRE(s.own_units * (s.cluster > 1 ? s.cluster : 1) + s.pre_blocks < (int64_t(1) << 31) &&
+                    int64_t(s.rows_blk) * a.p.kv_heads * a.p.seqs < (int64_t(1) << 31),
+                std::string(name) + ": sizes out of range");
+    const Scratch w = scratch_of(a.p, s, hd);
+    const size_t need = w.bytes;
     if (want) {
         *want = need;
         return VOX_CUDA_OK;
     }
     const int64_t el = 16 / dtype_size(dtype);
-    VOX_REQUIRE(q && out, nm + ": NULL pointer");
-    VOX_REQUIRE(prefix_len == 0 || prefix_pages, nm + ": NULL prefix_pages");
+    VOX_REQUIRE(q && out, std::string(name) + ": NULL pointer");
+    VOX_REQUIRE(prefix_len == 0 || prefix_pages, std::string(name) + ": NULL prefix_pages");
     VOX_REQUIRE(q_stride >= heads * hd && out_stride >= heads * hd && q_stride % el == 0 && out_stride % el == 0 && aligned16(q) && aligned16(out),
-                nm + ": q and out must be 16-byte aligned, their row strides cover a row in multiples of 16 bytes");
+                std::string(name) + ": q and out must be 16-byte aligned, their row strides cover a row in multiples of 16 bytes");
     VOX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
-                nm + ": workspace too small or not 256-byte aligned (vox_cuda_attn_workspace)");
+                std::string(name) + ": workspace too small or not 256-byte aligned (vox_cuda_attn_workspace)");
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.prefix_pages = prefix_pages, a.prefix_len = int32_t(prefix_len);
     a.window = int32_t(window < (int64_t(1) << 30) ? window : 0);
@@ -322,15 +318,17 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.gdiv = FastDiv(uint32_t(a.p.group));
     a.own_splits = s.own_splits, a.own_chunk = s.own_chunk, a.own_tiles = s.own_tiles;
     a.pre_splits = s.pre_splits, a.pre_chunk = s.pre_chunk, a.pre_tiles = s.pre_tiles;
-    a.kvdiv = FastDiv(uint32_t(a.p.kv_heads)), a.otdiv = FastDiv(uint32_t(s.own_tiles)), a.osdiv = FastDiv(uint32_t(s.own_splits));
-    a.ptdiv = FastDiv(uint32_t(s.pre_tiles > 0 ? s.pre_tiles : 1));
-    a.splits = s.own_splits + s.pre_splits;
+    auto div_by = [](int d) { return FastDiv(uint32_t(d > 0 ? d : 1)); };
+    a.kvdiv = div_by(a.p.kv_heads), a.otdiv = div_by(s.own_tiles), a.osdiv = div_by(s.own_splits), a.ptdiv = div_by(s.pre_tiles);
+    a.splits = s.slots, a.partial = w.partial;
     a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
     a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;
     a.tc_rows = s.tc_rows, a.concat = s.concat;
-    const size_t slots = size_t(a.p.tokens) * size_t(heads) * size_t(a.splits);
-    a.part_o = static_cast<float *>(workspace);
-    a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + slots * size_t(hd) * sizeof(float));
+    a.cluster = s.cluster, a.stream_keys = s.stream_keys, a.stream_rows = s.stream_rows, a.stream_rb = s.rows_blk;
+    a.stream_blocks = int32_t(s.frame == kFrameStream ? s.own_units : 0);
+    char *scratch = static_cast<char *>(workspace);
+    a.part_o = reinterpret_cast<float *>(scratch), a.part_ml = reinterpret_cast<float2 *>(scratch + w.part_ml);
+    a.stream_o = reinterpret_cast<float *>(scratch + w.stream_o), a.stream_ml = reinterpret_cast<float2 *>(scratch + w.stream_ml);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     using bf = __nv_bfloat16;
     const bool qf = dtype == VOX_CUDA_F32;
@@ -342,18 +340,17 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
         if (r != VOX_CUDA_OK) return r;
     }
     if (s.own_tc) {
-        r = attn_tc_launch(a, *cache, s.own_blocks, st, name);
+        r = attn_tc_launch(a, *cache, s.own_units, st, name);
     } else {
         a.pre_blocks = s.pre_tc ? 0 : int32_t(s.pre_blocks);
-        const int64_t n = a.pre_blocks + s.own_blocks;
+        const int64_t n = a.pre_blocks + s.own_units;
         if (s.mma)
-            r = attn_mma_launch(a, hd, s.rows_blk, dtype, n, st, name);
-        else if (hd == 64)
-            r = qf ? launch_vec<float, 64>(a, s, n, st, name) : launch_vec<bf, 64>(a, s, n, st, name);
+            r = attn_mma_launch(a, hd, s.rows_blk, dtype, s.frame, n, st, name);
         else
-            r = qf ? launch_vec<float, 128>(a, s, n, st, name) : launch_vec<bf, 128>(a, s, n, st, name);
+            r = with_vec(dtype, hd, s.rows_blk, [&](auto core) { return launch_rows<decltype(core)>(a, s.frame, n, st, name); });
+        if (s.frame != kFrameGrid) return r;  // joined there
     }
-    if (r != VOX_CUDA_OK || a.splits == 1) return r;
+    if (r != VOX_CUDA_OK || !a.partial) return r;
     if (hd == 64) return qf ? launch_merge<float, 64>(a, st, name) : launch_merge<bf, 64>(a, st, name);
     return qf ? launch_merge<float, 128>(a, st, name) : launch_merge<bf, 128>(a, st, name);
 }

@@ -26,18 +26,27 @@ struct AttnArgs {
     // the prefix: likewise, over the rows of all tokens
     int32_t pre_splits, pre_chunk, pre_tiles;
     FastDiv kvdiv, otdiv, osdiv, ptdiv;        // divisions by kv_heads, own_tiles, own_splits, pre_tiles
-    int32_t pre_blocks, splits;                // blocks of the prefix (they come first); pre_splits + own_splits
+    int32_t pre_blocks, splits;                // blocks of the prefix (they come first); slots of a row in the workspace
+    int32_t partial;                           // results go to the workspace (a row's parts meet in a later launch)
     // the tensor-core kernel: rows a block; whether this launch takes the prefix; whether the own keys follow the prefix
     // in one walk (then pre_splits is 0). own_tiles counts the row tiles of all sequences there.
     int32_t tc_rows, tc_prefix, concat;
     // there the scale is positive (row maxima are taken before it): a negative one flips q's signs, zero clears q
     float tc_scale;
     uint32_t q_and, q_xor;
-    float *part_o;                             // [tokens * heads][splits][hd], splits > 1
+    // few query rows (attn_rows.cuh): blocks a cluster; or keys a tile of the list, rows that the joining launch looks at,
+    // rows and number of the parts, and the parts themselves
+    int32_t cluster, stream_keys, stream_rows, stream_rb, stream_blocks;
+    float *stream_o;
+    float2 *stream_ml;
+    float *part_o;                             // [tokens * heads][splits][hd]
     float2 *part_ml;                           // [tokens * heads][splits]: (maximum, sum)
 };
 
-// A block's job, the same in every kernel.
+// Which frame of attn_rows.cuh takes a part of a call.
+enum RowsFrame { kFrameGrid = 0, kFrameCluster = 1, kFrameStream = 2 };
+
+// A block's job (rows x keys).
 struct AttnJob {
     int tok0, rows;        // first token; rows = tokens of the job * group
     int kvh;
@@ -88,8 +97,9 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
 }
 
 
-// Few rows on a bf16 cache (attn_mma.cu): rows_blk 8, or 16 (bf16 activations).
-int attn_mma_launch(const AttnArgs &a, int head_dim, int rows_blk, int dtype, int64_t blocks, cudaStream_t st, const char *name);
+// Few rows on a bf16 cache (attn_mma.cu): rows_blk 8, or 16 (bf16 activations); units: blocks, or clusters.
+int attn_mma_launch(AttnArgs &a, int head_dim, int rows_blk, int dtype, int frame, int64_t units, cudaStream_t st, const char *name);
+int attn_mma_resident(int head_dim, int rows_blk, int dtype);  // blocks of the stream frame on the device at once
 // The tensor-core path (attn_tc.cu).
 int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name);
 

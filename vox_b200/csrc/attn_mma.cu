@@ -1,0 +1,308 @@
+// The paged attention of few query rows on a bf16 cache (single tokens, short continuations; f32 activations of any
+// count): bound by reading K and V once, so the products only have to stay out of the way of the loads.
+//
+// A warp takes 16 keys a step (32 of 64-wide heads) against 8 or 16 rows, everything in registers: K and V go from global
+// memory straight into the operand registers of mma.m16n8k16, with no shared memory in between. That works because the
+// order of a product's summation index is free: S^T = K Q^T sums over the head's elements, so lane (g, t) may supply of key
+// g the 16-byte chunks t, t + 4, .. as they lie in memory, if Q's operand takes the same chunks; and O^T = V^T P^T has V's
+// elements as its rows, so lane (g, t) loads the chunks g, g + 8 of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs two keys'
+// halves with one byte permute. The weights turn from S^T's layout (lane: a key, two rows) to P^T's (lane: a row, two keys)
+// by one 8 x 8 transpose in registers. The softmax keeps one reference maximum a row for the warp, moved only when a score
+// exceeds it by 8 (base 2), so that the common step has one vote and no reduction.
+//
+// f32 activations keep f32 accuracy on the bf16 tensor cores: q and the weights are each cut into three bf16 parts (8 + 8 +
+// 8 significant bits), whose products with the bf16 keys and values are exact and accumulate in f32 in the same registers;
+// a step's P V is added to the running output by f32 additions rounded to nearest.
+#include "attn_rows.cuh"
+
+namespace voxcuda {
+namespace {
+
+// D += A . B, m16n8k16, bf16 operands, f32 accumulator.
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// (x, y) cut into PIECES bf16 pairs whose sums are x and y (3 pieces: to 24 significant bits).
+template <int PIECES>
+__device__ __forceinline__ void cut_bf16(float x, float y, uint32_t (&w)[PIECES]) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        w[p] = pack_bf16(x, y);
+        x -= bf16lo(w[p]);
+        y -= bf16hi(w[p]);
+    }
+}
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+template <typename QT, int HD_, int NT>
+struct MmaCore {
+    using Q = QT;
+    static constexpr int HD = HD_, RB = 8 * NT;
+    static constexpr int kMinBlocks = sizeof(QT) == 4 || NT == 2 ? 2 : 3;
+
+    static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB]) {
+        constexpr int PIECES = sizeof(QT) == 4 ? 3 : 1;
+        constexpr int KT = HD == 128 ? 1 : 2;       // runs of 16 keys a step
+        constexpr int KC = HD / 32, VC = HD / 64;   // 16-byte chunks a lane takes of a key of K, of a key of V
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row0 = j.row0;
+        const __nv_bfloat16 *K = static_cast<const __nv_bfloat16 *>(a.p.k) + int64_t(j.kvh) * a.p.head_stride;
+        const __nv_bfloat16 *V = static_cast<const __nv_bfloat16 *>(a.p.v) + int64_t(j.kvh) * a.p.head_stride;
+        // Q^T operand: row g of each n-tile, chunk t + 4 c, words 2 h and 2 h + 1 for the two products of a chunk
+        uint32_t q[NT][PIECES][KC][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int rr = row0 + 8 * n + g;
+            const int i = int(a.gdiv.div(uint32_t(min(rr, j.rows - 1)))), h = j.kvh * a.p.group + min(rr, j.rows - 1) - i * a.p.group;
+            const QT *src = static_cast<const QT *>(a.q) + int64_t(j.tok0 + i) * a.q_stride + int64_t(h) * HD;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                if constexpr (PIECES == 1) {
+                    const uint4 v = ld_param(src + (t + 4 * c) * 8);
+                    q[n][0][c][0] = v.x, q[n][0][c][1] = v.y, q[n][0][c][2] = v.z, q[n][0][c][3] = v.w;
+                } else {
+                    const float4 u0 = as_f4(ld_param(src + (t + 4 * c) * 8)), u1 = as_f4(ld_param(src + (t + 4 * c) * 8 + 4));
+                    const float f[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t pc[PIECES];
+                        cut_bf16<PIECES>(f[2 * w], f[2 * w + 1], pc);
+#pragma unroll
+                        for (int p = 0; p < PIECES; ++p) q[n][p][c][w] = pc[p];
+                    }
+                }
+            }
+        }
+        // softmax state of rows 2 t, 2 t + 1 of each n-tile; the keys that they see, and those that every row sees
+        float ref[NT][2], l[NT][2];
+        int hi[NT][2], lo[NT][2];
+        int kmin = j.k1, kend = j.k0, all_lo = j.k0, all_hi = j.k1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int rr = min(row0 + 8 * n + 2 * t + e, j.rows - 1), i = int(a.gdiv.div(uint32_t(rr)));
+                ref[n][e] = -INFINITY, l[n][e] = 0.f;
+                hi[n][e] = j.causal ? min(j.base + i + 1, j.k1) : j.k1;
+                lo[n][e] = a.window > 0 && j.causal ? max(j.base + i + 1 - a.window, j.k0) : j.k0;
+            }
+        {   // over the block's rows: tokens ascend, so the first row sees the earliest keys and the last row the latest
+            const int i0 = int(a.gdiv.div(uint32_t(row0))), i1 = int(a.gdiv.div(uint32_t(min(row0 + RB, j.rows) - 1)));
+            if (j.causal) {
+                all_hi = min(j.base + i0 + 1, j.k1), kend = min(j.base + i1 + 1, j.k1);
+                if (a.window > 0) kmin = max(j.base + i0 + 1 - a.window, j.k0), all_lo = max(j.base + i1 + 1 - a.window, j.k0);
+                else kmin = j.k0;
+            } else {
+                kmin = j.k0, kend = j.k1;
+            }
+        }
+        float acc[VC][4][NT][4];
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) acc[i][e][n][x] = 0.f;
+
+        uint4 kr[KT][2][KC], vr[KT][4][VC];
+        constexpr int STEP = 16 * KT * kRowsWarps;
+        const int first = (kmin & ~15) + warp * 16 * KT;
+        // page of the 16 keys from `key` on (they never leave one: pages are 16 rows or more)
+        auto page_of = [&](int key) { return key < kend ? __ldg(j.pages + (key >> a.p.page_shift)) : 0; };
+        auto offset = [&](int key, int page) {
+            return key < kend ? int64_t(page_checked(a.p, page)) * a.p.page_stride + int64_t(key & a.p.page_mask) * a.p.row_stride : int64_t(0);
+        };
+        auto load_k = [&](int base, const int64_t (&off)[KT]) {
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                const int kb = base + 16 * u;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int d = g + 8 * r;
+                    const __nv_bfloat16 *src = K + off[u] + int64_t(d) * a.p.row_stride + t * 8;
+                    const bool in = kb + d >= kmin && kb + d < kend;
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) kr[u][r][c] = in ? ld_stream(src + 32 * c) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        };
+        auto load_v = [&](int base, const int64_t (&off)[KT]) {
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                const int kb = base + 16 * u;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = 2 * t + (r & 1) + 8 * (r >> 1);
+                    const __nv_bfloat16 *src = V + off[u] + int64_t(d) * a.p.row_stride + g * 8;
+                    const bool in = kb + d >= kmin && kb + d < kend;  // rows outside are never read: they may hold anything
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) vr[u][r][c] = in ? ld_stream(src + 64 * c) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        };
+        int64_t off[KT];
+        int next[KT];
+#pragma unroll
+        for (int u = 0; u < KT; ++u) off[u] = offset(first + 16 * u, page_of(first + 16 * u));
+        load_k(first, off);
+        load_v(first, off);
+#pragma unroll
+        for (int u = 0; u < KT; ++u) next[u] = page_of(first + STEP + 16 * u);
+        for (int base = first; base < kend; base += STEP) {
+            // S^T: keys g and g + 8 (registers 0-1, 2-3) of rows 2 t, 2 t + 1
+            float s[KT][NT][4];
+#pragma unroll
+            for (int u = 0; u < KT; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    // independent chains: one a part of q, or one a half of the chunks' words
+                    constexpr int CH = PIECES == 1 ? 2 : PIECES;
+                    float d[CH][4];
+#pragma unroll
+                    for (int y = 0; y < CH; ++y)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) d[y][x] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int p = 0; p < PIECES; ++p)
+                                mma16816(d[PIECES == 1 ? h : p], word(kr[u][0][c], 2 * h), word(kr[u][1][c], 2 * h), word(kr[u][0][c], 2 * h + 1),
+                                         word(kr[u][1][c], 2 * h + 1), q[n][p][c][2 * h], q[n][p][c][2 * h + 1]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[u][n][x] = PIECES == 1 ? d[0][x] + d[1][x] : (d[CH - 1][x] + d[1][x]) + d[0][x];
+                }
+            // the next step's K, and its page after that
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                off[u] = offset(base + STEP + 16 * u, next[u]);
+                next[u] = page_of(base + 2 * STEP + 16 * u);
+            }
+            load_k(base + STEP, off);
+            const bool mask = base < all_lo || base + 16 * KT > all_hi;
+            bool move = false;
+#pragma unroll
+            for (int u = 0; u < KT; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        s[u][n][x] *= a.scale_log2;
+                        if (mask) {
+                            const int key = base + 16 * u + g + 8 * (x >> 1);
+                            if (key < lo[n][x & 1] || key >= hi[n][x & 1]) s[u][n][x] = -INFINITY;
+                        }
+                        move = move || s[u][n][x] > ref[n][x & 1] + 8.0f;  // also a row's first key (ref = -inf)
+                    }
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < KT; ++u) mx = fmaxf(mx, fmaxf(s[u][n][e], s[u][n][e + 2]));
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        if (mx > ref[n][e]) {
+                            const float alpha = ex2_approx(ref[n][e] - mx);
+                            ref[n][e] = mx;
+                            l[n][e] *= alpha;
+#pragma unroll
+                            for (int i = 0; i < VC; ++i)
+#pragma unroll
+                                for (int f = 0; f < 4; ++f) acc[i][f][n][e] *= alpha, acc[i][f][n][e + 2] *= alpha;
+                        }
+                    }
+            }
+            uint32_t pf[KT][NT][PIECES][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float r0 = ref[n][0] == -INFINITY ? 0.f : ref[n][0], r1 = ref[n][1] == -INFINITY ? 0.f : ref[n][1];
+#pragma unroll
+                for (int u = 0; u < KT; ++u)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float p0 = ex2_approx(s[u][n][2 * x] - r0), p1 = ex2_approx(s[u][n][2 * x + 1] - r1);
+                        l[n][0] += p0, l[n][1] += p1;
+                        uint32_t w[PIECES];
+                        cut_bf16<PIECES>(p0, p1, w);
+#pragma unroll
+                        for (int p = 0; p < PIECES; ++p) pf[u][n][p][x] = transpose8x8(w[p]);
+                    }
+            }
+            // O^T += V^T P^T: elements 8 (g + 8 i) + 2 e (registers 0-1) and + 1 (2-3) of rows 2 t, 2 t + 1
+#pragma unroll
+            for (int i = 0; i < VC; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float d[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) d[n][x] = PIECES == 1 ? acc[i][e][n][x] : 0.f;
+#pragma unroll
+                    for (int u = 0; u < KT; ++u) {
+                        const uint32_t w0 = word(vr[u][0][i], e), w1 = word(vr[u][1][i], e), w2 = word(vr[u][2][i], e), w3 = word(vr[u][3][i], e);
+                        const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+                        const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int p = PIECES - 1; p >= 0; --p) mma16816(d[n], a0, a1, a2, a3, pf[u][n][p][0], pf[u][n][p][1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[i][e][n][x] = PIECES == 1 ? d[n][x] : acc[i][e][n][x] + d[n][x];
+                }
+            load_v(base + STEP, off);
+        }
+        // the warps' parts of each row
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+                if (g == 0) s_ml[warp][8 * n + 2 * t + e] = make_float2(ref[n][e], l[n][e]);
+#pragma unroll
+                for (int i = 0; i < VC; ++i)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                        *reinterpret_cast<float2 *>(&s_acc[warp][8 * n + 2 * t + e][8 * (g + 8 * i) + 2 * f]) =
+                            make_float2(acc[i][f][n][e], acc[i][f][n][e + 2]);
+            }
+    }
+};
+
+template <typename F>
+int with_core(int head_dim, int rows_blk, int dtype, F f) {
+    using bf = __nv_bfloat16;
+    if (dtype == VOX_CUDA_F32) return head_dim == 64 ? f(MmaCore<float, 64, 1>()) : f(MmaCore<float, 128, 1>());
+    if (rows_blk > 8) return head_dim == 64 ? f(MmaCore<bf, 64, 2>()) : f(MmaCore<bf, 128, 2>());
+    return head_dim == 64 ? f(MmaCore<bf, 64, 1>()) : f(MmaCore<bf, 128, 1>());
+}
+
+}  // namespace
+
+int attn_mma_launch(AttnArgs &a, int head_dim, int rows_blk, int dtype, int frame, int64_t units, cudaStream_t st, const char *name) {
+    return with_core(head_dim, rows_blk, dtype, [&](auto core) { return launch_rows<decltype(core)>(a, frame, units, st, name); });
+}
+int attn_mma_resident(int head_dim, int rows_blk, int dtype) {
+    return with_core(head_dim, rows_blk, dtype,
+                     [](auto core) { return resident_blocks((const void *)attn_stream_kernel<decltype(core)>, kRowsThreads, 0); });
+}
+
+int attn_mma_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+
+}  // namespace voxcuda

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int h = j.kvh * a.p.group + (live ? rr - i_tok * a.p.group : 0);
         const int64_t tok = j.tok0 + i_tok;
         const int64_t slot = (tok * a.p.heads + h) * a.splits + j.split;
-        const float inv = a.splits > 1 ? 1.0f : l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
+        const float inv = a.partial ? 1.0f : l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
         __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + tok * a.out_stride + int64_t(h) * HD;
         float *pdst = a.part_o + slot * HD;
 #pragma unroll
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int e = 0; e < 32; ++e) o[e] = 0;
             }
             if (!live || !ok) continue;
-            if (a.splits > 1) {
+            if (a.partial) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)
                     *reinterpret_cast<uint4 *>(pdst + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
         }
-        if (live && ok && a.splits > 1) a.part_ml[slot] = make_float2(ref, l);
+        if (live && ok && a.partial) a.part_ml[slot] = make_float2(ref, l);
     } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {

@@ -160,26 +160,25 @@ int launch_append(AppendArgs &a, cudaStream_t st) {
 }  // namespace
 
 int paged_args(const vox_cuda_kv_cache *c, const vox_cuda_kv_batch *b, int64_t heads, const char *name, PagedArgs &a) {
-    const std::string nm(name);
-    VOX_REQUIRE(c && b, nm + ": NULL cache or batch");
-    VOX_REQUIRE(is_act_dtype(c->dtype), nm + ": the cache must be f32 or bf16");
+    VOX_REQUIRE(c && b, std::string(name) + ": NULL cache or batch");
+    VOX_REQUIRE(is_act_dtype(c->dtype), std::string(name) + ": the cache must be f32 or bf16");
     VOX_REQUIRE(c->page_size >= 16 && c->page_size <= (1 << 20) && (c->page_size & (c->page_size - 1)) == 0,
-                nm + ": page_size must be a power of two, 16 to 2^20");
+                std::string(name) + ": page_size must be a power of two, 16 to 2^20");
     VOX_REQUIRE(c->pages > 0 && c->kv_heads > 0 && heads > 0 && heads % c->kv_heads == 0 && heads <= 65535,
-                nm + ": bad cache shape (heads must be a multiple of kv_heads)");
-    if (c->head_dim != 64 && c->head_dim != 128) return set_error(VOX_CUDA_ERR_UNSUPPORTED, nm + ": head_dim must be 64 or 128");
+                std::string(name) + ": bad cache shape (heads must be a multiple of kv_heads)");
+    if (c->head_dim != 64 && c->head_dim != 128) return set_error(VOX_CUDA_ERR_UNSUPPORTED, std::string(name) + ": head_dim must be 64 or 128");
     const int64_t el = 16 / dtype_size(c->dtype);
     VOX_REQUIRE(c->page_stride % el == 0 && c->row_stride % el == 0 && c->head_stride % el == 0 && c->page_stride >= 0 && c->row_stride > 0 &&
                     c->head_stride > 0,
-                nm + ": cache strides must be positive multiples of 16 bytes");
+                std::string(name) + ": cache strides must be positive multiples of 16 bytes");
     VOX_REQUIRE(b->seqs >= 0 && b->tokens >= 0 && b->table_width >= 0 && b->table_stride >= b->table_width && b->max_q >= 0 && b->max_kv >= 0,
-                nm + ": bad batch shape");
+                std::string(name) + ": bad batch shape");
     VOX_REQUIRE(b->tokens * heads < (int64_t(1) << 31) && int64_t(b->table_width) * c->page_size <= (int64_t(1) << 30),
-                nm + ": sizes out of range");
+                std::string(name) + ": sizes out of range");
     if (b->seqs == 0 || b->tokens == 0) return VOX_CUDA_OK;
-    VOX_REQUIRE(c->k && c->v && (b->page_table || b->table_width == 0) && b->kv_len, nm + ": NULL pointer");
-    VOX_REQUIRE(aligned16(c->k) && aligned16(c->v), nm + ": the cache must be 16-byte aligned");
-    VOX_REQUIRE(b->q_start || b->tokens % b->seqs == 0, nm + ": without q_start the tokens must be a multiple of seqs");
+    VOX_REQUIRE(c->k && c->v && (b->page_table || b->table_width == 0) && b->kv_len, std::string(name) + ": NULL pointer");
+    VOX_REQUIRE(aligned16(c->k) && aligned16(c->v), std::string(name) + ": the cache must be 16-byte aligned");
+    VOX_REQUIRE(b->q_start || b->tokens % b->seqs == 0, std::string(name) + ": without q_start the tokens must be a multiple of seqs");
     a.k = c->k, a.v = c->v, a.table = b->page_table, a.kv_len = b->kv_len, a.q_start = b->q_start;
     a.table_stride = b->table_stride, a.page_stride = c->page_stride, a.row_stride = c->row_stride, a.head_stride = c->head_stride;
     a.page_mask = c->page_size - 1;

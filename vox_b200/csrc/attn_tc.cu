@@ -27,28 +27,64 @@ namespace {
 
 constexpr int kKeys = 128;
 constexpr int kTcThreads = 384;
-constexpr int kTcRegs = 168;  // registers a thread at launch; 2 x 224 + 56 = 3 x 168 after the split below
+constexpr int kTcRegs = 168;  // registers a thread at launch; 2 x 200 + 104 = 3 x 168 after the split below
 constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 
 constexpr int tc_stages(int hd) { return hd == 128 ? 5 : 8; }
 constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }
 
-// D[tmem] (+)= A[tmem] . B[smem], issued by one elected lane of a converged warp (A: 128 lanes, two bf16 a column).
-__device__ __forceinline__ void umma_bf16_ta_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+// The products of one tile, issued by one elected lane of a converged warp in one piece of code (the issuing warp runs once
+// a tile between long stretches of softmax code, so its instructions are cold: few of them matter).
+// S = Q K^T: HD / 16 steps; both operands K-major, 32 bytes a step, the second 64 elements kHalf bytes on.
+template <int HD>
+__device__ __forceinline__ void umma_qk_warp(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint64_t *bar) {
+#define VOX_QK_STEP(OFF, P) "add.s64 a, %1, " OFF ";\n\tadd.s64 b, %2, " OFF ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, " P ";\n\t"
+#define VOX_QK_HEAD "{\n\t.reg .pred e, z, o;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 z, 0, 0;\n\tsetp.eq.b32 o, 0, 0;\n\t"
+#define VOX_COMMIT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}"
+    if constexpr (HD == 128)
+        asm volatile(VOX_QK_HEAD VOX_QK_STEP("0", "z") VOX_QK_STEP("2", "o") VOX_QK_STEP("4", "o") VOX_QK_STEP("6", "o") VOX_QK_STEP("1024", "o")
+                         VOX_QK_STEP("1026", "o") VOX_QK_STEP("1028", "o") VOX_QK_STEP("1030", "o") VOX_COMMIT ::"r"(d),
+                     "l"(da), "l"(db), "r"(idesc), "r"(smem_addr(bar))
+                     : "memory");
+    else
+        asm volatile(VOX_QK_HEAD VOX_QK_STEP("0", "z") VOX_QK_STEP("2", "o") VOX_QK_STEP("4", "o") VOX_QK_STEP("6", "o") VOX_COMMIT ::"r"(d), "l"(da),
+                     "l"(db), "r"(idesc), "r"(smem_addr(bar))
+                     : "memory");
+}
+// O (+)= P V, 16 keys a step: P in TMEM (two bf16 a column: 8 columns a step), V MN-major (2048 bytes a step). The first six
+// steps (acc: whether O holds something), and the last two.
+#define VOX_PV_STEP(C, OFF, P) "add.s32 a, %1, " C ";\n\tadd.s64 b, %2, " OFF ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, " P ";\n\t"
+__device__ __forceinline__ void umma_pv_first_warp(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred e, p, o;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 o, 0, 0;\n\t"
+                 VOX_PV_STEP("0", "0", "p") VOX_PV_STEP("8", "128", "o") VOX_PV_STEP("16", "256", "o") VOX_PV_STEP("24", "384", "o")
+                 VOX_PV_STEP("32", "512", "o") VOX_PV_STEP("40", "640", "o") "}" ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_pv_rest_warp(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc) {
+    asm volatile("{\n\t.reg .pred e, o;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.eq.b32 o, 0, 0;\n\t"
+                 VOX_PV_STEP("48", "768", "o") VOX_PV_STEP("56", "896", "o") "}" ::"r"(d), "r"(ta), "l"(db), "r"(idesc)
+                 : "memory");
 }
 // 16 consecutive columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// mbar_wait_warp with the timer and the limit (a load from memory) kept out of the first polls: the waits of this kernel
+// last a few hundred clocks, and a poll that comes late by such a load delays the whole chain of products and softmax.
+__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return mbar_wait_warp(bar, parity);
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+    return d;
+}
 // Tiled tensor copy of a 4-D map's box; x times the element size is a multiple of 128 bytes at every call site.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -138,14 +174,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sQ = smem_addr(smem), sKV = sQ + 2 * kTile;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + (2 + NS) * kTile), *empty = full + NS;
-    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *tail = o_full + 2, *drain = tail + 1;
+    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *p_rest = p_full + 2, *o_full = p_rest + 2, *tail = o_full + 2, *drain = tail + 1;
     uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_enter();
     if (warp == 0) tc_job(a, blockIdx.x, job);
     if (threadIdx.x == 32) {
         for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int q = 0; q < 2; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 128), mbar_init(&o_full[q], 1);
+        for (int q = 0; q < 2; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 4), mbar_init(&p_rest[q], 4), mbar_init(&o_full[q], 1);
         mbar_init(tail, 1);
         mbar_init(drain, 1);
         mbar_init_fence();
@@ -199,7 +235,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if (warp < 8) {
         // ---------------------------------------------------------------- softmax: thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int q = warp >> 2, row = (warp & 3) * 32 + lane, rr = j.row0 + 128 * q + row;
         const int n = q ? nt[1] : nt[0];
         const uint32_t tS = tmem + (uint32_t((warp & 3) * 32) << 16) + 128 * q, tP = tS + 64;
@@ -209,10 +245,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int hi_own = live && j.causal ? min(j.base + i_tok + 1, j.k1) : 0;
         const int lo_own = a.window > 0 ? max(j.base + i_tok + 1 - a.window, j.k0) : j.k0;
         float ref = -INFINITY;  // reference maximum (scaled, base 2)
-        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
-            ok = mbar_wait_warp(&s_full[q], uint32_t(i & 1));
+            ok = wait_soon(&s_full[q], uint32_t(i & 1));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[128];
@@ -228,16 +264,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int c = 0; c < kKeys; ++c)
                     if (c >= hi || c < lo) r[c] = __float_as_uint(-INFINITY);
             }
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float m8[8];
 #pragma unroll
-            for (int c = 0; c < kKeys; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(r[c]));
-            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.tc_scale;
+            for (int c = 0; c < 8; ++c) m8[c] = max3(__uint_as_float(r[c]), __uint_as_float(r[c + 8]), __uint_as_float(r[c + 16]));
+#pragma unroll
+            for (int c = 24; c < kKeys - 8; c += 16)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m8[e] = max3(m8[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 8 + e]));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m8[e] = fmaxf(m8[e], __uint_as_float(r[kKeys - 8 + e]));
+            const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * a.tc_scale;
             const bool move = mx > ref + 8.0f;  // also the first key that the row sees (ref = -inf)
             if (__any_sync(0xffffffffu, move)) {
                 const float nref = move ? mx : ref;
                 const float alpha = move ? ex2_approx(ref - nref) : 1.0f;
                 ref = nref;
-                l2[0] = mul2(l2[0], bc2(alpha)), l2[1] = mul2(l2[1], bc2(alpha));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l2[e] = mul2(l2[e], bc2(alpha));
                 if (i > 0) {  // the arrival of this S implies that the P V before it has completed
 #pragma unroll
                     for (int c = 0; c < HD / 16; ++c) {
@@ -267,20 +310,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int k = 32 * c + 2 * e;
                     const float2 x = fma2(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc, nr);
                     const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                    l2[e & 1] = add2(l2[e & 1], p);
+                    l2[e & 3] = add2(l2[e & 3], p);
                     w[e] = pack_bf16(p.x, p.y);
                 }
                 tmem_st16(tP + 16 * c, w);
+                if (c >= 2) {  // three quarters of the weights, then the rest: the second product starts on what is there
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c == 2 ? &p_full[q] : &p_rest[q]);
+                }
             }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[q]);
         }
         if (n > 0 && ok) {
-            ok = mbar_wait_warp(&o_full[q], 0);
+            ok = wait_soon(&o_full[q], 0);
             tc_fence_after();
         }
-        const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+        const float2 ls = add2(add2(l2[0], l2[1]), add2(l2[2], l2[3]));
+        const float l = ls.x + ls.y;
         const int h = j.kvh * a.p.group + (live ? rr - i_tok * a.p.group : 0);
         const int64_t tok = j.tok0 + i_tok;
         const int64_t slot = (tok * a.p.heads + h) * a.splits + j.split;
@@ -314,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (live && ok && a.partial) a.part_ml[slot] = make_float2(ref, l);
     } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 8) {
         // ---------------------------------------------------------------- copies
         const int pr = min(a.p.page_mask + 1, kKeys);  // rows a box
@@ -325,7 +372,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool is_v = n & 1, pre = i < nA;
             const int key0 = pre ? j.pa0 + i * kKeys : kb0 + (i - nA) * kKeys;
             const int valid = min((pre ? j.pa1 : kend) - key0, kKeys);
-            if (n >= NS) ok = mbar_wait_warp(&empty[s], uint32_t(n / NS - 1) & 1u);
+            if (n >= NS) ok = wait_soon(&empty[s], uint32_t(n / NS - 1) & 1u);
             if (!ok) break;
             const int boxes = (valid + pr - 1) / pr * H;
             const bool zero = is_v && valid < kKeys;
@@ -339,7 +386,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tma_load_4d(st + half * kHalf + p * pr * 128, is_v ? &mv : &mk, half * 64, j.kvh, key & a.p.page_mask, page, bar);
             }
             if (zero) {
-                ok = mbar_wait_warp(tail, uint32_t(tails++ & 1));
+                ok = wait_soon(tail, uint32_t(tails++ & 1));
                 for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
 #pragma unroll
                     for (int half = 0; half < H; ++half)
@@ -350,62 +397,55 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         // every copy issued has landed before the block's shared memory is released
-        for (int m = max(n - NS, 0); m < n; ++m) mbar_wait_warp(&full[m % NS], uint32_t(m / NS) & 1u);
+        for (int m = max(n - NS, 0); m < n; ++m) wait_soon(&full[m % NS], uint32_t(m / NS) & 1u);
     } else if (warp == 9) {
         // ---------------------------------------------------------------- MMAs
         bool ok = true;
-        auto wait_full = [&](int m) { return mbar_wait_warp(&full[m % NS], uint32_t(m / NS) & 1u); };
-        auto qk = [&](int q, int m) {
-            const uint32_t tQ = sQ + q * kTile, tK = sKV + (m % NS) * kTile;
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-                umma_bf16_warp(tmem + 128 * q, umma_desc(tQ + off, 16, 1024), umma_desc(tK + off, 16, 1024), kIdS, k > 0);
-            }
-            umma_commit_warp(&s_full[q]);
-        };
+        auto wait_full = [&](int m) { return wait_soon(&full[m % NS], uint32_t(m / NS) & 1u); };
+        const uint64_t dQ = umma_desc(sQ, 16, 1024), dK = umma_desc(sKV, 16, 1024), dV = umma_desc(sKV, kHalf, 1024);
+        constexpr uint32_t kStep = kTile >> 4;  // a tile on, in descriptor units
+        auto qk = [&](int q, int st) { umma_qk_warp<HD>(tmem + 128 * q, dQ + uint32_t(q) * kStep, dK + uint32_t(st) * kStep, kIdS, &s_full[q]); };
         if (nmax > 0) {
             ok = wait_full(0);
             tc_fence_after();
             if (ok) {
+#pragma unroll 1
                 for (int q = 0; q < 2; ++q)
-                    if (nt[q] > 0) qk(q, 0);
+                    if ((q ? nt[1] : nt[0]) > 0) qk(q, 0);
                 umma_commit_warp(&empty[0]);
             }
         }
+#pragma unroll 1
         for (int i = 0; i < nmax && ok; ++i) {
-            const int mv_ = 2 * i + 1, mk_ = 2 * i + 2;
-            bool vw = false, kw = false;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                if (i >= nt[q] || !ok) continue;
-                ok = mbar_wait_warp(&p_full[q], uint32_t(i & 1));
-                if (ok && !vw) ok = wait_full(mv_);
-                vw = true;
-                if (!ok) continue;
+            const int nv = 2 * i + 1, sv = nv % NS, sk = (nv + 1) % NS;
+            ok = wait_full(nv);  // V of this tile, usually there long before P
+            if (i + 1 < nmax) ok = ok && wait_full(nv + 1);
+#pragma unroll 1
+            for (int q = 0; q < 2 && ok; ++q) {
+                const int n = q ? nt[1] : nt[0];
+                if (i >= n) continue;
+                const uint32_t tO = tmem + 256 + HD * q, tP = tmem + 128 * q + 64;
+                ok = wait_soon(&p_full[q], uint32_t(i & 1));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t tV = sKV + (mv_ % NS) * kTile;
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)  // 16 keys a step: 8 columns of P, 16 rows (2048 bytes) of V
-                    umma_bf16_ta_warp(tmem + 256 + HD * q, tmem + 128 * q + 64 + 8 * k, umma_desc(tV + 2048 * k, kHalf, 1024), kIdO,
-                                      uint32_t(i > 0 || k > 0));
-                if (i + 1 == nt[q]) umma_commit_warp(&o_full[q]);
-                if (i + 1 < nt[q]) {
-                    if (!kw) ok = wait_full(mk_);
-                    kw = true;
-                    if (!ok) continue;
-                    tc_fence_after();
-                    qk(q, mk_);
-                }
+                umma_pv_first_warp(tO, tP, dV + uint32_t(sv) * kStep, kIdO, uint32_t(i > 0));
+                ok = wait_soon(&p_rest[q], uint32_t(i & 1));
+                if (!ok) break;
+                tc_fence_after();
+                umma_pv_rest_warp(tO, tP, dV + uint32_t(sv) * kStep, kIdO);
+                if (i + 1 < n)
+                    qk(q, sk);
+                else
+                    umma_commit_warp(&o_full[q]);
             }
             if (ok) {
-                umma_commit_warp(&empty[mv_ % NS]);
-                if (i + 1 < nmax) umma_commit_warp(&empty[mk_ % NS]);
+                umma_commit_warp(&empty[sv]);
+                if (i + 1 < nmax) umma_commit_warp(&empty[sk]);
             }
         }
         umma_commit_warp(drain);  // every MMA issued has completed before the tensor memory is released
         __syncwarp();
-        mbar_wait_warp(drain, 0);
+        wait_soon(drain, 0);
     }
     }
     tc_fence_before();

@@ -72,13 +72,21 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// mbar_wait_warp with the timer and the limit (a load from memory) kept out of the first polls: the waits of this kernel
-// last a few hundred clocks, and a poll that comes late by such a load delays the whole chain of products and softmax.
+// Bounded wait of a converged warp, as mbar_wait_warp, in little code whose first 256 polls touch neither the timer nor
+// memory: the waits of this kernel last a few hundred clocks, and its warps share their instruction caches.
 __device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity) {
+    uint64_t t0 = 0;
 #pragma unroll 1
-    for (int i = 0; i < 256; ++i)
+    for (uint32_t i = 1;; ++i) {
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return mbar_wait_warp(bar, parity);
+        if ((i & 255u) == 0) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (__any_sync(0xffffffffu, now - t0 > kWaitLimitNs)) break;
+        }
+    }
+    if ((threadIdx.x & 31) == 0) atomicOr(&g_device_error, kDevErrTimeout);
+    return false;
 }
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float d;
@@ -174,22 +182,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sQ = smem_addr(smem), sKV = sQ + 2 * kTile;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + (2 + NS) * kTile), *empty = full + NS;
-    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *p_rest = p_full + 2, *o_full = p_rest + 2, *tail = o_full + 2, *drain = tail + 1;
+    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *p_rest = p_full + 2, *o_full = p_rest + 2, *q_full = o_full + 2, *tail = q_full + 2, *drain = tail + 1;
     uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_enter();
     if (warp == 0) tc_job(a, blockIdx.x, job);
     if (threadIdx.x == 32) {
         for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int q = 0; q < 2; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 4), mbar_init(&p_rest[q], 4), mbar_init(&o_full[q], 1);
+        for (int q = 0; q < 2; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 4), mbar_init(&p_rest[q], 4), mbar_init(&q_full[q], 4), mbar_init(&o_full[q], 1);
         mbar_init(tail, 1);
         mbar_init(drain, 1);
         mbar_init_fence();
     }
-    __syncthreads();
-    const TcJob j = job;
-    if (!j.ok) return;
     if (warp == 9) tmem_alloc(tslot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const TcJob j = job;
+    const uint32_t tmem = *tslot;
+    if (!j.ok) {
+        if (warp == 9) tmem_dealloc(tmem, 512);
+        return;
+    }
     // key tiles: nA of the prefix, then the own keys from kb0; hi of a row tile = keys that its last row sees
     const int nA = (j.pa1 - j.pa0 + kKeys - 1) / kKeys;
     int kb0 = j.k0;
@@ -210,32 +224,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
     const int nmax = max(nt[0], nt[1]);
-    if (warp < 8) {  // Q tiles: 16-byte chunks of whole rows, 128-byte swizzle; rows past the end are zero
-        const int q = warp >> 2, w = warp & 3;
-        const uint32_t tQ = sQ + q * kTile;
-        constexpr int CH = HD / 8, RPI = 32 / CH;  // chunks a row, rows a warp step
-#pragma unroll 4
-        for (int s = 0; s < 32 / RPI; ++s) {
-            const int r = w * 32 + s * RPI + lane / CH, c = lane % CH, rr = j.row0 + 128 * q + r;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (rr < j.rows && nt[q] > 0) {
-                const int i = int(a.gdiv.div(uint32_t(rr))), h = j.kvh * a.p.group + rr - i * a.p.group;
-                v = ld_stream(static_cast<const __nv_bfloat16 *>(a.q) + int64_t(j.tok0 + i) * a.q_stride + int64_t(h) * HD + c * 8);
-            }
-            v.x = (v.x & a.q_and) ^ a.q_xor, v.y = (v.y & a.q_and) ^ a.q_xor, v.z = (v.z & a.q_and) ^ a.q_xor, v.w = (v.w & a.q_and) ^ a.q_xor;
-            const uint32_t dst = tQ + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-        }
-        fence_proxy_async();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tslot;
-
     if (warp < 8) {
         // ---------------------------------------------------------------- softmax: thread = row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        {   // the row tile's Q: 16-byte chunks of whole rows, every load in flight before the first is stored, 128-byte
+            // swizzle; rows past the end are zero
+            const int q = warp >> 2, w = warp & 3;
+            const uint32_t tQ = sQ + q * kTile;
+            constexpr int CH = HD / 8, RPI = 32 / CH;  // chunks a row, rows a warp step
+            uint4 v[32 / RPI];
+#pragma unroll
+            for (int s = 0; s < 32 / RPI; ++s) {
+                const int rr = j.row0 + 128 * q + w * 32 + s * RPI + lane / CH;
+                v[s] = make_uint4(0, 0, 0, 0);
+                if (rr < j.rows && (q ? nt[1] : nt[0]) > 0) {
+                    const int i = int(a.gdiv.div(uint32_t(rr))), h = j.kvh * a.p.group + rr - i * a.p.group;
+                    v[s] = ld_param(static_cast<const __nv_bfloat16 *>(a.q) + int64_t(j.tok0 + i) * a.q_stride + int64_t(h) * HD + lane % CH * 8);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 32 / RPI; ++s) {
+                const int r = w * 32 + s * RPI + lane / CH, c = lane % CH;
+                const uint32_t dst = tQ + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"((v[s].x & a.q_and) ^ a.q_xor),
+                             "r"((v[s].y & a.q_and) ^ a.q_xor), "r"((v[s].z & a.q_and) ^ a.q_xor), "r"((v[s].w & a.q_and) ^ a.q_xor)
+                             : "memory");
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[q]);
+        }
         const int q = warp >> 2, row = (warp & 3) * 32 + lane, rr = j.row0 + 128 * q + row;
         const int n = q ? nt[1] : nt[0];
         const uint32_t tS = tmem + (uint32_t((warp & 3) * 32) << 16) + 128 * q, tP = tS + 64;
@@ -410,8 +428,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
             if (ok) {
 #pragma unroll 1
-                for (int q = 0; q < 2; ++q)
-                    if ((q ? nt[1] : nt[0]) > 0) qk(q, 0);
+                for (int q = 0; q < 2 && ok; ++q)
+                    if ((q ? nt[1] : nt[0]) > 0) {
+                        ok = wait_soon(&q_full[q], 0);
+                        tc_fence_after();
+                        if (ok) qk(q, 0);
+                    }
                 umma_commit_warp(&empty[0]);
             }
         }

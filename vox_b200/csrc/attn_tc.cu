@@ -30,6 +30,8 @@ constexpr int kTcThreads = 384;
 constexpr int kTcRegs = 168;  // registers a thread at launch; 2 x 200 + 104 = 3 x 168 after the split below
 constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 
+constexpr int POLY = 0x10;  // which of eight pairs of weights take ex2_poly
+
 constexpr int tc_stages(int hd) { return hd == 128 ? 5 : 8; }
 constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }
 
@@ -92,6 +94,21 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
     return d;
+}
+// 2^x for x <= 64 or so on the multiply-add pipe (two elements), beside the 16 results a clock of the special-function unit:
+// x = n + f, n the nearest integer (from the low bits of x + 1.5 2^23), 2^f by a cubic whose relative error on
+// [-1/2, 1/2] is below 7.5e-5 (a least-maximum fit made for this kernel; the weights are rounded to bf16 next, 2^-8), times 2^n
+// built from its exponent bits. Below -126 (masked scores too) it gives 2^-126; NaN stays NaN.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    const float2 t = add2(x, bc2(12582912.0f));
+    const float2 f = add2(x, fma2(t, bc2(-1.0f), bc2(12582912.0f)));
+    float2 p = fma2(bc2(0.05517132f), f, bc2(0.24261054f));
+    p = fma2(p, f, bc2(0.69326099f));
+    p = fma2(p, f, bc2(0.99992811f));
+    return mul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3F800000u),
+                               __uint_as_float((__float_as_uint(t.y) << 23) + 0x3F800000u)));
 }
 // Tiled tensor copy of a 4-D map's box; x times the element size is a multiple of 128 bytes at every call site.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
@@ -327,7 +344,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int e = 0; e < 16; ++e) {
                     const int k = 32 * c + 2 * e;
                     const float2 x = fma2(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc, nr);
-                    const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    // part of the weights on the multiply-add pipe: the special-function unit alone would take all of a tile
+                    const float2 p = (POLY >> (e & 7)) & 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
                     l2[e & 3] = add2(l2[e & 3], p);
                     w[e] = pack_bf16(p.x, p.y);
                 }
@@ -345,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
         }
         const float2 ls = add2(add2(l2[0], l2[1]), add2(l2[2], l2[3]));
-        const float l = ls.x + ls.y;
+        const float l = ref == -INFINITY && ls.x + ls.y < 1.0f ? 0.f : ls.x + ls.y;  // a row that saw no key (a NaN sum stays)
         const int h = j.kvh * a.p.group + (live ? rr - i_tok * a.p.group : 0);
         const int64_t tok = j.tok0 + i_tok;
         const int64_t slot = (tok * a.p.heads + h) * a.splits + j.split;

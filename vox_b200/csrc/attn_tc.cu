@@ -368,32 +368,59 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t tok = j.tok0 + i_tok;
         const int64_t slot = (tok * a.p.heads + h) * a.splits + j.split;
         const float inv = a.partial ? 1.0f : l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
-        __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + tok * a.out_stride + int64_t(h) * HD;
-        float *pdst = a.part_o + slot * HD;
+        // a warp's 32 rows go through the row tile's Q (its products are complete) so that they are stored in whole runs of a
+        // row: 64 columns a pass of the f32 parts, all of a row a pass of the bf16 result (one 16-byte chunk a lane, the
+        // chunks of a row swizzled over the banks)
+        constexpr int CPR = HD / 8;  // chunks of a row a pass
+        const uint32_t stage = sQ + q * kTile + (warp & 3) * (kTile / 4);
+        char *dst = a.partial ? reinterpret_cast<char *>(a.part_o + slot * HD)
+                              : reinterpret_cast<char *>(static_cast<__nv_bfloat16 *>(a.out) + tok * a.out_stride + int64_t(h) * HD);
+        if (!live || !ok) dst = nullptr;
+        auto put = [&](int c, uint4 v) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * (CPR * 16) + ((c ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z),
+                         "r"(v.w)
+                         : "memory");
+        };
+        const int passes = a.partial ? 2 : 1;
+#pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass) {
+            const int cols = a.partial ? HD / 2 : HD;
+#pragma unroll 1
+            for (int col = 0; col < cols; col += 32) {
+                uint32_t o[32];
+                if (n > 0 && ok) {
+                    tmem_ld32(tO + pass * (HD / 2) + col, o);
+                    tmem_wait_ld(o);
+                } else {
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            if (n > 0 && ok) {
-                tmem_ld32(tO + 32 * c, o);
-                tmem_wait_ld(o);
-            } else {
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (a.partial) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0;
-            }
-            if (!live || !ok) continue;
-            if (a.partial) {
+                    for (int c = 0; c < 8; ++c) put(col / 4 + c, make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
+                } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    *reinterpret_cast<uint4 *>(pdst + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            } else {
+                    for (int c = 0; c < 4; ++c) {
+                        float f[8];
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    float f[8];
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(o[e + u]) * inv;
-                    *reinterpret_cast<uint4 *>(dst + 32 * c + e) = Vec<VOX_CUDA_BF16>::pack(f);
+                        for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(o[8 * c + u]) * inv;
+                        put(col / 8 + c, Vec<VOX_CUDA_BF16>::pack(f));
+                    }
                 }
             }
+            __syncwarp();
+#pragma unroll 4
+            for (int x = 0; x < CPR; ++x) {  // CPR lanes a row, 32 / CPR rows a step
+                const int r = x * (32 / CPR) + lane / CPR, c = lane % CPR;
+                char *to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+                uint4 v;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                             : "r"(stage + r * (CPR * 16) + ((c ^ (r & 7)) << 4))
+                             : "memory");
+                if (to != nullptr) *reinterpret_cast<uint4 *>(to + pass * (CPR * 16) + c * 16) = v;
+            }
+            __syncwarp();
         }
         if (live && ok && a.partial) a.part_ml[slot] = make_float2(ref, l);
     } else {

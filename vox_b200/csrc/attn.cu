@@ -259,18 +259,21 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
 // The workspace: the slots of every row (where a row has more than one, or its own keys are taken by another frame), then
 // the parts of the stream frame. Offsets in bytes; returns the size.
 struct Scratch {
-    size_t part_ml, stream_o, stream_ml, bytes;
+    size_t part_ml, stream_o, stream_ml, stream_desc, bytes;
     bool partial;
 };
 Scratch scratch_of(const PagedArgs &p, const AttnShape &s, int head_dim) {
     Scratch w = {};
     w.partial = s.slots > 1 || (s.pre_splits > 0 && s.own_splits == 0);
     const size_t slots = w.partial ? size_t(p.tokens) * size_t(p.heads) * size_t(s.slots) : 0;
-    const size_t parts = s.own_splits == 0 && s.frame == kFrameStream ? size_t(s.own_units) * 2 * size_t(s.rows_blk) : 0;
+    const bool stream = s.own_splits == 0 && s.frame == kFrameStream;
+    const size_t heads = size_t(p.seqs) * size_t(p.kv_heads);  // a sequence's key/value heads
+    const size_t parts = stream ? (size_t(s.own_units) * 2 + (s.pre_splits > 0 ? heads : 0)) * size_t(s.rows_blk) : 0;
     w.part_ml = slots * size_t(head_dim) * sizeof(float);
     w.stream_o = (w.part_ml + slots * sizeof(float2) + 255) & ~size_t(255);
     w.stream_ml = w.stream_o + parts * size_t(head_dim) * sizeof(float);
-    w.bytes = w.stream_ml + parts * sizeof(float2);
+    w.stream_desc = w.stream_ml + parts * sizeof(float2);
+    w.bytes = w.stream_desc + (stream ? heads * sizeof(int2) : 0);
     return w;
 }
 
@@ -329,6 +332,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     char *scratch = static_cast<char *>(workspace);
     a.part_o = reinterpret_cast<float *>(scratch), a.part_ml = reinterpret_cast<float2 *>(scratch + w.part_ml);
     a.stream_o = reinterpret_cast<float *>(scratch + w.stream_o), a.stream_ml = reinterpret_cast<float2 *>(scratch + w.stream_ml);
+    a.stream_desc = reinterpret_cast<int2 *>(scratch + w.stream_desc);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     using bf = __nv_bfloat16;
     const bool qf = dtype == VOX_CUDA_F32;

@@ -39,6 +39,7 @@ struct AttnArgs {
     int32_t cluster, stream_keys, stream_rows, stream_rb, stream_blocks;
     float *stream_o;
     float2 *stream_ml;
+    int2 *stream_desc;  // [seqs][kv_heads]: first and last block of a sequence's tiles
     float *part_o;                             // [tokens * heads][splits][hd]
     float2 *part_ml;                           // [tokens * heads][splits]: (maximum, sum)
 };

@@ -244,164 +244,183 @@ __device__ __forceinline__ int64_t stream_total(const AttnArgs &a, int64_t (&par
     return total;
 }
 
+// Where a block stands in the list, kept in shared memory: the registers belong to the core.
+struct StreamState {
+    int64_t u, u1, start, total;  // next tile, end of the block's run, first tile of sequence b, all tiles
+    int b, tiles, extra;
+    RowsJob job;
+    int part;                     // of the workspace; -1: the rows are stored
+};
+
 template <class Core>
 __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_kernel(const AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
     __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
-    __shared__ int64_t s_part[kRowsThreads], s_start;
-    __shared__ int s_seq;
+    __shared__ int64_t s_part[kRowsThreads];
+    __shared__ StreamState st;
     pdl_enter();
-    const int64_t c = blockIdx.x;
-    int64_t u, u1, start;
-    int b;
     {
         int64_t before;
         int b0, b1;
-        const int64_t total = stream_total(a, s_part, before, b0, b1);
+        const int64_t c = blockIdx.x, total = stream_total(a, s_part, before, b0, b1);
         const int64_t blocks = min(int64_t(gridDim.x), total);  // no block without a tile between two that share a sequence
         if (c >= blocks) return;
-        u = total * c / blocks, u1 = total * (c + 1) / blocks;
+        const int64_t u = total * c / blocks;
+        if (threadIdx.x == 0) st.u = u, st.u1 = total * (c + 1) / blocks, st.total = total, st.extra = 0;
         for (int x = b0; x < b1; ++x) {  // the thread whose sequences hold tile u
             int t, n, kv, lo;
-            const int64_t w = int64_t(stream_tiles(a, x, t, n, kv, lo)) * a.p.kv_heads;
-            if (u >= before && u < before + w) s_seq = x, s_start = before;
+            const int tiles = stream_tiles(a, x, t, n, kv, lo);
+            const int64_t w = int64_t(tiles) * a.p.kv_heads;
+            if (u >= before && u < before + w) st.b = x, st.start = before, st.tiles = tiles;
             before += w;
         }
         __syncthreads();
-        b = s_seq, start = s_start;
     }
-    int tok0, n, kv, lo, extra = 0;
-    int tiles = stream_tiles(a, b, tok0, n, kv, lo);
-    while (u < u1) {
-        while (u >= start + int64_t(tiles) * a.p.kv_heads) {
-            start += int64_t(tiles) * a.p.kv_heads;
-            tiles = stream_tiles(a, ++b, tok0, n, kv, lo);
-        }
-        const int kvh = int((u - start) / tiles);
-        const int64_t s0 = start + int64_t(kvh) * tiles;  // the list positions of this sequence and head: s0 .. s0 + tiles
-        const int64_t e = min(s0 + tiles, u1);
-        const bool head = u == s0, whole = head && e == s0 + tiles;
-        const int rows = n * a.p.group;
-        // rows past RB (a sequence with more new tokens than the host's bound): the block of the first tile takes them over
-        // all keys
-        const int row0 = extra * RB;
-        const int k0 = extra ? lo : min(lo + int(u - s0) * a.stream_keys, kv), k1 = extra ? kv : min(lo + int(e - s0) * a.stream_keys, kv);
-        Core::run(a, RowsJob{tok0, rows, row0, kvh, kv - n, true, k0, k1, a.p.table + int64_t(b) * a.p.table_stride}, s_acc, s_ml);
-        __syncthreads();
-        for (int x = threadIdx.x; x < RB * (HD / 4); x += kRowsThreads) {
-            const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
-            if (row0 + r >= rows) break;
-            Join t = join_warps<RB, HD>(s_acc, s_ml, r, d);
-            int tok, h;
-            row_of(a, tok0, kvh, row0 + r, tok, h);
-            if (whole || extra) {
-                if (a.pre_splits > 0) {
-                    Join p;
-                    add_prefix<HD>(a, p, tok, h, d);
-                    p.add(t.m, t.l, t.o);
-                    t = p;
+    for (;;) {
+        if (threadIdx.x == 0) {
+            int64_t u = st.u, start = st.start;
+            int b = st.b, tiles = st.tiles, tok0, n, kv, lo;
+            const int extra = st.extra;
+            if (u < st.u1) {
+                tiles = stream_tiles(a, b, tok0, n, kv, lo);
+                while (u >= start + int64_t(tiles) * a.p.kv_heads) {
+                    start += int64_t(tiles) * a.p.kv_heads;
+                    tiles = stream_tiles(a, ++b, tok0, n, kv, lo);
                 }
-                store4(static_cast<typename Core::Q *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
+                const int kvh = int((u - start) / tiles);
+                const int64_t s0 = start + int64_t(kvh) * tiles;  // the list positions of this sequence and head: s0 .. s0 + tiles
+                const int64_t e = min(s0 + tiles, st.u1);
+                const bool head = u == s0, whole = head && e == s0 + tiles;
+                const int rows = n * a.p.group;
+                // rows past RB (a sequence with more new tokens than the host's bound): the block of the first tile takes them
+                // over all keys
+                st.job = RowsJob{tok0, rows, extra * RB, kvh, kv - n, true, extra ? lo : min(lo + int(u - s0) * a.stream_keys, kv),
+                                 extra ? kv : min(lo + int(e - s0) * a.stream_keys, kv), a.p.table + int64_t(b) * a.p.table_stride};
+                st.part = (whole && a.pre_splits == 0) || extra ? -1 : whole ? 2 * a.stream_blocks + b * a.p.kv_heads + kvh : 2 * int(blockIdx.x) + (head ? 1 : 0);
+                // the blocks that share this sequence and head: block of tile u is the c with total c / blocks <= u < total (c + 1)
+                // / blocks (rounded down)
+                const int64_t blocks = min(int64_t(gridDim.x), st.total);
+                if (head) a.stream_desc[int64_t(b) * a.p.kv_heads + kvh] = make_int2(int(blockIdx.x), int(((s0 + tiles) * blocks - 1) / st.total));
+                const bool more = head && (extra + 1) * RB < rows;
+                st.extra = more ? extra + 1 : 0;
+                st.u = more ? u : e;
+                st.start = start, st.b = b, st.tiles = tiles;
             } else {
-                const int64_t slot = (2 * c + (head ? 1 : 0)) * RB + r;
-                store4(a.stream_o + slot * HD + d, t.o);
-                if (d == 0) a.stream_ml[slot] = make_float2(t.m, t.l);
+                st.job.tok0 = -1;
             }
         }
         __syncthreads();
-        if (head && (extra + 1) * RB < rows) {
-            ++extra;
-        } else {
-            extra = 0;
-            u = e;
-        }
-    }
-}
-
-// One block a sequence and query-head row: joins the parts of the blocks that share its keys; rows that one block took
-// whole are stored already. Grid: (rows of a sequence up to RB) * kv_heads * seqs.
-template <typename QT, int HD>
-__global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const AttnArgs a) {
-    __shared__ int64_t s_part[kRowsThreads], s_total, s_before;
-    __shared__ float s_o[kRowsWarps][HD];
-    __shared__ float2 s_ml[kRowsWarps];
-    pdl_enter();
-    const int r = int(blockIdx.x % uint32_t(a.stream_rows));
-    const uint32_t y = blockIdx.x / uint32_t(a.stream_rows), b = a.kvdiv.div(y);
-    const int kvh = int(y - b * uint32_t(a.p.kv_heads));
-    {
-        int64_t before;
-        int b0, b1;
-        const int64_t total = stream_total(a, s_part, before, b0, b1);
-        for (int x = b0; x < b1; ++x) {
-            int t, n, kv, lo;
-            const int64_t w = int64_t(stream_tiles(a, x, t, n, kv, lo)) * a.p.kv_heads;
-            if (x == int(b)) s_before = before, s_total = total;
-            before += w;
+        if (st.job.tok0 < 0) return;
+        Core::run(a, st.job, s_acc, s_ml);
+        __syncthreads();
+        const RowsJob j = st.job;
+        const int64_t part = st.part;
+        for (int x = threadIdx.x; x < RB * (HD / 4); x += kRowsThreads) {
+            const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
+            if (j.row0 + r >= j.rows) break;
+            Join t = join_warps<RB, HD>(s_acc, s_ml, r, d);
+            if (part >= 0) {
+                store4(a.stream_o + (part * RB + r) * HD + d, t.o);
+                if (d == 0) a.stream_ml[part * RB + r] = make_float2(t.m, t.l);
+                continue;
+            }
+            int tok, h;
+            row_of(a, j.tok0, j.kvh, j.row0 + r, tok, h);
+            if (a.pre_splits > 0) {
+                Join p;
+                add_prefix<HD>(a, p, tok, h, d);
+                p.add(t.m, t.l, t.o);
+                t = p;
+            }
+            store4(static_cast<typename Core::Q *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
         }
         __syncthreads();
     }
+}
+
+// One block a sequence and query-head row: joins the parts of the shared prefix and of the blocks that share the
+// sequence's keys; rows that one block took whole are stored already (without a prefix). Warp w takes parts w, w + 4, ..,
+// lane: elements E lane .. of the row. Grid: (rows of a sequence up to RB) * kv_heads * seqs.
+template <typename QT, int HD>
+__global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const AttnArgs a) {
+    constexpr int E = HD / 32;
+    __shared__ __align__(16) float s_o[kRowsWarps][HD];
+    __shared__ float2 s_ml[kRowsWarps];
+    pdl_enter();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = int(blockIdx.x % uint32_t(a.stream_rows));
+    const uint32_t y = blockIdx.x / uint32_t(a.stream_rows), b = a.kvdiv.div(y);
+    const int kvh = int(y - b * uint32_t(a.p.kv_heads));
+    const int2 desc = __ldcg(a.stream_desc + y);
     int tok0, n, kv, lo;
     const int tiles = stream_tiles(a, int(b), tok0, n, kv, lo);
     const int rows = n * a.p.group;
     if (r >= rows) return;
-    const int64_t total = s_total, blocks = min(int64_t(a.stream_blocks), total);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int tok, h;
-    int64_t c0 = 0, c1 = -1;
+    int own = 0, c0 = 0;
     if (tiles > 0) {
-        // block of tile u: the c with total c / blocks <= u < total (c + 1) / blocks (rounded down)
-        const int64_t s0 = s_before + int64_t(kvh) * tiles, s1 = s0 + tiles - 1;
-        auto block_of = [&](int64_t u) { return ((u + 1) * blocks - 1) / total; };
-        c0 = block_of(s0), c1 = block_of(s1);
-        if (c0 == c1) return;  // stored by its block
-    } else {
-        for (int rr = r + a.stream_rows; rr < rows; rr += a.stream_rows) {  // rows past the bound of a sequence without keys
-            row_of(a, tok0, kvh, rr, tok, h);
-            for (int d = threadIdx.x * 4; d < HD; d += kRowsThreads * 4) {
-                Join t;
-                add_prefix<HD>(a, t, tok, h, d);
-                store4(static_cast<QT *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
+        c0 = desc.x, own = desc.y - desc.x + 1;
+        if (own == 1 && a.pre_splits == 0) return;
+    }
+    // a sequence without keys: this launch alone stores its rows, those past the host's bound too
+    for (int row = r; row < (tiles > 0 ? r + 1 : rows); row += a.stream_rows) {
+        int tok, h;
+        row_of(a, tok0, kvh, row, tok, h);
+        const int64_t pre = (int64_t(tok) * a.p.heads + h) * a.splits;
+        const int parts = a.pre_splits + own, mine = (parts - warp + kRowsWarps - 1) / kRowsWarps;
+        // part p: a slot of the prefix, or the c0-th, .. block's part of the own keys (kept as a whole where there is one)
+        auto slot = [&](int p, const float2 *&ml, const float *&o) {
+            if (p < a.pre_splits) {
+                ml = a.part_ml + pre + p, o = a.part_o + (pre + p) * HD;
+                return;
+            }
+            const int c = c0 + p - a.pre_splits;
+            const int64_t part = own == 1 ? 2 * int64_t(a.stream_blocks) + y : 2 * int64_t(c) + (c == c0 ? 1 : 0);
+            ml = a.stream_ml + part * a.stream_rb + r, o = a.stream_o + (part * a.stream_rb + r) * HD;
+        };
+        float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+        for (int base = 0; base < mine; base += 32) {
+            const int cnt = min(mine - base, 32);
+            const float2 *ml;
+            const float *po;
+            slot(warp + (base + min(lane, cnt - 1)) * kRowsWarps, ml, po);
+            const float2 v = lane < cnt ? __ldcg(ml) : make_float2(-INFINITY, 0.f);
+            const float mx = fmaxf(m, warp_max(v.x)), ms = mx == -INFINITY ? 0.f : mx;
+            const float alpha = ex2_approx(m - ms), w = ex2_approx(v.x - ms);
+            m = mx;
+            l = l * alpha + warp_sum(v.x == -INFINITY ? v.y : v.y * w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= alpha;
+            for (int k = 0; k < cnt; k += 4) {  // four parts in flight
+                float x[4][E];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(po), min(k + u, cnt - 1)));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[u][e] = __ldcg(src + lane * E + e);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float wu = __shfl_sync(0xffffffffu, w, min(k + u, 31));
+                    if (k + u < cnt)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o[e] = fmaf(x[u][e], wu, o[e]);
+                }
             }
         }
-    }
-    // warp w joins a contiguous quarter of the parts, lane: elements E lane .. of the row
-    constexpr int E = HD / 32;
-    const int64_t cnt = c1 - c0 + 1, per = (cnt + kRowsWarps - 1) / kRowsWarps;
-    float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    auto add = [&](float pm, float pl, const float *po) {
-        if (pm == -INFINITY) {
-            l += pl;
-            return;
+        for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+        if (lane == 0) s_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        for (int d = threadIdx.x * 4; d < HD; d += kRowsThreads * 4) {
+            Join t;
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) t.add(s_ml[w].x, s_ml[w].y, *reinterpret_cast<const float4 *>(&s_o[w][d]));
+            store4(static_cast<QT *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
         }
-        const float mx = fmaxf(m, pm), wa = ex2_approx(m - mx), wb = ex2_approx(pm - mx);
-        m = mx;
-        l = l * wa + pl * wb;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * wa + po[e] * wb;
-    };
-    for (int64_t c = c0 + warp * per; c < min(c0 + (warp + 1) * per, c1 + 1); ++c) {
-        const int64_t slot = (2 * c + (c == c0 ? 1 : 0)) * a.stream_rb + r;
-        const float2 ml = __ldcg(a.stream_ml + slot);
-        float po[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) po[e] = __ldcg(a.stream_o + slot * HD + lane * E + e);
-        add(ml.x, ml.y, po);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-    if (lane == 0) s_ml[warp] = make_float2(m, l);
-    __syncthreads();
-    row_of(a, tok0, kvh, r, tok, h);
-    for (int d = threadIdx.x * 4; d < HD; d += kRowsThreads * 4) {
-        Join t;
-        add_prefix<HD>(a, t, tok, h, d);
-#pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) t.add(s_ml[w].x, s_ml[w].y, *reinterpret_cast<const float4 *>(&s_o[w][d]));
-        store4(static_cast<QT *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
+        __syncthreads();
     }
 }
 

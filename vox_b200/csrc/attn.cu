@@ -20,8 +20,14 @@ template <typename QT, int HD_, int R>
 struct VecCore {
     using Q = QT;
     static constexpr int HD = HD_, RB = R, kMinBlocks = R <= 4 ? 4 : 2;
+    static constexpr size_t kSmem = 0;
+    struct State {};
+    static __device__ __forceinline__ void init(State &) {}
 
-    static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB]) {
+
+    template <typename F>
+    static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB], State &, F between) {
+        between();
         constexpr int V = 4;                        // elements a lane holds of a key
         constexpr int LPK = HD / V, KPW = 32 / LPK; // lanes a key, keys a warp load
         constexpr int U = R <= 2 ? 8 : 4;           // loads of K (and of V) in flight
@@ -187,7 +193,7 @@ struct AttnShape {
     int rows_blk, tc_rows;
     int own_tiles, own_splits, own_chunk;
     int pre_tiles, pre_splits, pre_chunk;
-    int cluster, stream_keys, stream_rows;
+    int cluster, stream_shift, stream_rows;
     int64_t own_units, pre_blocks;     // blocks, or clusters
     int slots;                         // of a row in the workspace
 };
@@ -226,13 +232,11 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         const int64_t own = int64_t(s.own_tiles) * p.kv_heads;
         cut_keys(max_kv, s.concat ? 1 : own < sms ? sms / own : 1, s.own_splits, s.own_chunk);
         s.own_units = own * s.own_splits;
-    } else if (rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc)) {
+    } else if (rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc) && base * ((int64_t(p.cap) >> 6) + 1) < (int64_t(1) << 31)) {
         // one row tile a sequence: a cluster for each sequence and key/value head where one wave of blocks holds them all
         // with at most 512 keys each, else equal runs of all sequences' tiles
         const int64_t resident = s.mma ? attn_mma_resident(head_dim, s.rows_blk, dtype)
-                                       : with_vec(dtype, head_dim, s.rows_blk, [](auto core) {
-                                             return resident_blocks((const void *)attn_stream_kernel<decltype(core)>, kRowsThreads, 0);
-                                         });
+                                       : with_vec(dtype, head_dim, s.rows_blk, [](auto core) { return rows_resident<decltype(core)>(); });
         int c = 8;
         while (c > 1 && (base * c > resident || 32 * c > max_kv)) c /= 2;
         if (base * c <= resident && max_kv <= 512 * c) {
@@ -241,9 +245,9 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
             s.own_units = base;
         } else {
             s.frame = kFrameStream;
-            s.stream_keys = head_dim == 64 ? 128 : 64;
+            s.stream_shift = head_dim == 64 ? 7 : 6;  // one step of a block's warps
             s.stream_rows = int(p.q_start ? s.rows_blk : rows);
-            const int64_t tiles = base * ((max_kv + s.stream_keys - 1) / s.stream_keys);
+            const int64_t tiles = base * ((max_kv + (1 << s.stream_shift) - 1) >> s.stream_shift);
             s.own_units = tiles < 1 ? 1 : tiles < resident ? tiles : resident;
         }
     } else {
@@ -327,7 +331,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
     a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;
     a.tc_rows = s.tc_rows, a.concat = s.concat;
-    a.cluster = s.cluster, a.stream_keys = s.stream_keys, a.stream_rows = s.stream_rows, a.stream_rb = s.rows_blk;
+    a.cluster = s.cluster, a.stream_shift = s.stream_shift, a.stream_rows = s.stream_rows, a.stream_rb = s.rows_blk;
     a.stream_blocks = int32_t(s.frame == kFrameStream ? s.own_units : 0);
     char *scratch = static_cast<char *>(workspace);
     a.part_o = reinterpret_cast<float *>(scratch), a.part_ml = reinterpret_cast<float2 *>(scratch + w.part_ml);
@@ -348,10 +352,14 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     } else {
         a.pre_blocks = s.pre_tc ? 0 : int32_t(s.pre_blocks);
         const int64_t n = a.pre_blocks + s.own_units;
-        if (s.mma)
+        if (s.mma) {
+            r = attn_cache_map(*cache, cache->k, 16, a.mk, name);
+            if (r == VOX_CUDA_OK) r = attn_cache_map(*cache, cache->v, 16, a.mv, name);
+            if (r != VOX_CUDA_OK) return r;
             r = attn_mma_launch(a, hd, s.rows_blk, dtype, s.frame, n, st, name);
-        else
+        } else {
             r = with_vec(dtype, hd, s.rows_blk, [&](auto core) { return launch_rows<decltype(core)>(a, s.frame, n, st, name); });
+        }
         if (s.frame != kFrameGrid) return r;  // joined there
     }
     if (r != VOX_CUDA_OK || !a.partial) return r;

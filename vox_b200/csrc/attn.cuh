@@ -8,6 +8,8 @@
 // (all exponents base 2: the scores are scaled by scale * log2 e before the softmax).
 #pragma once
 
+#include <cuda.h>
+
 #include "paged.cuh"
 
 namespace voxcuda {
@@ -34,11 +36,12 @@ struct AttnArgs {
     // there the scale is positive (row maxima are taken before it): a negative one flips q's signs, zero clears q
     float tc_scale;
     uint32_t q_and, q_xor;
-    // few query rows (attn_rows.cuh): blocks a cluster; or keys a tile of the list, rows that the joining launch looks at,
+    // few query rows (attn_rows.cuh): blocks a cluster; or log2 of the keys a tile of the list, rows that the joining launch looks at,
     // rows and number of the parts, and the parts themselves
-    int32_t cluster, stream_keys, stream_rows, stream_rb, stream_blocks;
+    int32_t cluster, stream_shift, stream_rows, stream_rb, stream_blocks;
     float *stream_o;
     float2 *stream_ml;
+    CUtensorMap mk, mv;  // the cache's tensors, boxes of 16 rows of one page (attn_mma.cu)
     int2 *stream_desc;  // [seqs][kv_heads]: first and last block of a sequence's tiles
     float *part_o;                             // [tokens * heads][splits][hd]
     float2 *part_ml;                           // [tokens * heads][splits]: (maximum, sum)
@@ -101,6 +104,31 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
 // Few rows on a bf16 cache (attn_mma.cu): rows_blk 8, or 16 (bf16 activations); units: blocks, or clusters.
 int attn_mma_launch(AttnArgs &a, int head_dim, int rows_blk, int dtype, int frame, int64_t units, cudaStream_t st, const char *name);
 int attn_mma_resident(int head_dim, int rows_blk, int dtype);  // blocks of the stream frame on the device at once
+// Map of one of the cache's tensors: [pages][page rows][kv heads][hd], box 64 elements of one head x box_rows rows of one
+// page, 128-byte swizzle (attn_tc.cu).
+int attn_cache_map(const vox_cuda_kv_cache &c, const void *base, int box_rows, CUtensorMap &m, const char *name);
+// Tiled tensor copy of such a map's box; x times the element size is a multiple of 128 bytes at every call site.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+                 : "memory");
+}
+// Bounded wait of a converged warp, as mbar_wait_warp, in little code whose first 256 polls touch neither the timer nor
+// memory: the waits of the attention kernels are short as a rule, and a poll that comes late delays all that follows it.
+__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity) {
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (uint32_t i = 1;; ++i) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if ((i & 255u) == 0) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (__any_sync(0xffffffffu, now - t0 > kWaitLimitNs)) break;
+        }
+    }
+    if ((threadIdx.x & 31) == 0) atomicOr(&g_device_error, kDevErrTimeout);
+    return false;
+}
 // The tensor-core path (attn_tc.cu).
 int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name);
 

@@ -1,9 +1,10 @@
 // The paged attention of few query rows on a bf16 cache (single tokens, short continuations; f32 activations of any
 // count): bound by reading K and V once, so the products only have to stay out of the way of the loads.
 //
-// A warp takes 16 keys a step (32 of 64-wide heads) against 8 or 16 rows, everything in registers: K and V go from global
-// memory straight into the operand registers of mma.m16n8k16, with no shared memory in between. That works because the
-// order of a product's summation index is free: S^T = K Q^T sums over the head's elements, so lane (g, t) may supply of key
+// A warp takes 16 keys a step (32 of 64-wide heads) against 8 or 16 rows. One lane has the tensor copy engine bring K and V
+// tiles of 16 keys x 128 bytes (a page or part of one) into the warp's own ring in shared memory, two steps ahead, so 16 KB a
+// warp are in flight at no cost in registers or issue slots; the lanes read 16-byte chunks back as operands of
+// mma.m16n8k16. Whole chunks serve as operands because the order of a product's summation index is free: S^T = K Q^T sums over the head's elements, so lane (g, t) may supply of key
 // g the 16-byte chunks t, t + 4, .. as they lie in memory, if Q's operand takes the same chunks; and O^T = V^T P^T has V's
 // elements as its rows, so lane (g, t) loads the chunks g, g + 8 of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs two keys'
 // halves with one byte permute. The weights turn from S^T's layout (lane: a key, two rows) to P^T's (lane: a row, two keys)
@@ -14,20 +15,26 @@
 // 8 significant bits), whose products with the bf16 keys and values are exact and accumulate in f32 in the same registers;
 // a step's P V is added to the running output by f32 additions rounded to nearest.
 #include "attn_rows.cuh"
+#include "tc.cuh"
 
 namespace voxcuda {
 namespace {
 
 // D += A . B, m16n8k16, bf16 operands, f32 accumulator.
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 // (x, y) cut into PIECES bf16 pairs whose sums are x and y (3 pieces: to 24 significant bits).
 template <int PIECES>
@@ -45,15 +52,84 @@ template <typename QT, int HD_, int NT>
 struct MmaCore {
     using Q = QT;
     static constexpr int HD = HD_, RB = 8 * NT;
-    static constexpr int kMinBlocks = sizeof(QT) == 4 || NT == 2 ? 2 : 3;
+    static constexpr int kMinBlocks = NT == 2 || sizeof(QT) == 4 ? 2 : 3;
+    static constexpr int kStages = 2;
+    static constexpr uint32_t kBox = 16 * 128;    // bytes of a box: 16 keys x 64 elements
+    static constexpr uint32_t kStage = 4 * kBox;  // K and V of a step: 2 halves of 16 keys, or 32 keys of 64-wide heads
+    static constexpr size_t kSmem = size_t(kRowsWarps) * kStages * kStage + 1024;
 
-    static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB]) {
+    // The warp's ring and its barriers; parity: bit s = parity of the next phase of stage s.
+    struct State {
+        uint32_t ring, parity;
+        uint64_t *bars;
+    };
+    static __device__ __forceinline__ void init(State &st) {
+        extern __shared__ uint8_t ring_raw[];
+        __shared__ uint64_t s_bars[kRowsWarps][kStages];
+        const int warp = threadIdx.x >> 5;
+        st.ring = ((smem_addr(ring_raw) + 1023u) & ~1023u) + uint32_t(warp) * kStages * kStage;
+        st.bars = s_bars[warp];
+        st.parity = 0;
+        if ((threadIdx.x & 31) == 0) {
+            for (int s = 0; s < kStages; ++s) mbar_init(&st.bars[s], 1);
+            mbar_init_fence();
+        }
+        __syncwarp();
+    }
+
+    template <typename F>
+    static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB], State &st, F between) {
         constexpr int PIECES = sizeof(QT) == 4 ? 3 : 1;
         constexpr int KT = HD == 128 ? 1 : 2;       // runs of 16 keys a step
         constexpr int KC = HD / 32, VC = HD / 64;   // 16-byte chunks a lane takes of a key of K, of a key of V
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row0 = j.row0;
-        const __nv_bfloat16 *K = static_cast<const __nv_bfloat16 *>(a.p.k) + int64_t(j.kvh) * a.p.head_stride;
-        const __nv_bfloat16 *V = static_cast<const __nv_bfloat16 *>(a.p.v) + int64_t(j.kvh) * a.p.head_stride;
+        // the keys that some row sees, and those that every row sees: tokens ascend, so the first row sees the earliest keys and
+        // the last row the latest
+        int kmin = j.k1, kend = j.k0, all_lo = j.k0, all_hi = j.k1;
+        {
+            const int i0 = int(a.gdiv.div(uint32_t(row0))), i1 = int(a.gdiv.div(uint32_t(min(row0 + RB, j.rows) - 1)));
+            if (j.causal) {
+                all_hi = min(j.base + i0 + 1, j.k1), kend = min(j.base + i1 + 1, j.k1);
+                if (a.window > 0) kmin = max(j.base + i0 + 1 - a.window, j.k0), all_lo = max(j.base + i1 + 1 - a.window, j.k0);
+                else kmin = j.k0;
+            } else {
+                kmin = j.k0, kend = j.k1;
+            }
+        }
+        constexpr int STEP = 16 * KT * kRowsWarps;
+        const int first = (kmin & ~15) + warp * 16 * KT;
+        // page of the 16 keys from `key` on (they never leave one: pages are 16 rows or more)
+        auto page_of = [&](int key) { return key < kend ? __ldg(j.pages + (key >> a.p.page_shift)) : 0; };
+        int next[KT];
+        // starts the copies of the step at `base` into a stage, then looks up the pages of the step after
+        auto issue = [&](int base, int stage) {
+            if (base >= kend) return;
+            const uint32_t to = st.ring + uint32_t(stage) * kStage;
+            uint64_t *bar = &st.bars[stage];
+            const int runs = KT == 1 || base + 16 >= kend ? 1 : 2;  // of 16 keys
+            if (lane == 0) mbar_arrive_expect_tx(bar, KT == 1 ? kStage : uint32_t(runs) * 2 * kBox);
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                if (u < runs) {
+                    const int kb = base + 16 * u, page = page_checked(a.p, next[u]);
+                    if (lane == 0) {
+#pragma unroll
+                        for (int h = 0; h < 2 / KT; ++h) {  // halves of a 128-wide head; x is a multiple of 128 bytes
+                            tma_load_4d(to + (u + h) * kBox, &a.mk, 64 * h, j.kvh, kb & a.p.page_mask, page, bar);
+                            tma_load_4d(to + (2 + u + h) * kBox, &a.mv, 64 * h, j.kvh, kb & a.p.page_mask, page, bar);
+                        }
+                    }
+                }
+                next[u] = page_of(base + STEP + 16 * u);
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < KT; ++u) next[u] = page_of(first + 16 * u);
+        __syncwarp();
+        if (lane == 0) fence_proxy_async();  // the ring was last read by ordinary loads
+#pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) issue(first + s * STEP, s);
+        between();
         // Q^T operand: row g of each n-tile, chunk t + 4 c, words 2 h and 2 h + 1 for the two products of a chunk
         uint32_t q[NT][PIECES][KC][4];
 #pragma unroll
@@ -79,10 +155,9 @@ struct MmaCore {
                 }
             }
         }
-        // softmax state of rows 2 t, 2 t + 1 of each n-tile; the keys that they see, and those that every row sees
+        // softmax state of rows 2 t, 2 t + 1 of each n-tile and the keys that they see
         float ref[NT][2], l[NT][2];
         int hi[NT][2], lo[NT][2];
-        int kmin = j.k1, kend = j.k0, all_lo = j.k0, all_hi = j.k1;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -92,16 +167,6 @@ struct MmaCore {
                 hi[n][e] = j.causal ? min(j.base + i + 1, j.k1) : j.k1;
                 lo[n][e] = a.window > 0 && j.causal ? max(j.base + i + 1 - a.window, j.k0) : j.k0;
             }
-        {   // over the block's rows: tokens ascend, so the first row sees the earliest keys and the last row the latest
-            const int i0 = int(a.gdiv.div(uint32_t(row0))), i1 = int(a.gdiv.div(uint32_t(min(row0 + RB, j.rows) - 1)));
-            if (j.causal) {
-                all_hi = min(j.base + i0 + 1, j.k1), kend = min(j.base + i1 + 1, j.k1);
-                if (a.window > 0) kmin = max(j.base + i0 + 1 - a.window, j.k0), all_lo = max(j.base + i1 + 1 - a.window, j.k0);
-                else kmin = j.k0;
-            } else {
-                kmin = j.k0, kend = j.k1;
-            }
-        }
         float acc[VC][4][NT][4];
 #pragma unroll
         for (int i = 0; i < VC; ++i)
@@ -112,59 +177,44 @@ struct MmaCore {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) acc[i][e][n][x] = 0.f;
 
-        uint4 kr[KT][2][KC], vr[KT][4][VC];
-        constexpr int STEP = 16 * KT * kRowsWarps;
-        const int first = (kmin & ~15) + warp * 16 * KT;
-        // page of the 16 keys from `key` on (they never leave one: pages are 16 rows or more)
-        auto page_of = [&](int key) { return key < kend ? __ldg(j.pages + (key >> a.p.page_shift)) : 0; };
-        auto offset = [&](int key, int page) {
-            return key < kend ? int64_t(page_checked(a.p, page)) * a.p.page_stride + int64_t(key & a.p.page_mask) * a.p.row_stride : int64_t(0);
-        };
-        auto load_k = [&](int base, const int64_t (&off)[KT]) {
-#pragma unroll
-            for (int u = 0; u < KT; ++u) {
-                const int kb = base + 16 * u;
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int d = g + 8 * r;
-                    const __nv_bfloat16 *src = K + off[u] + int64_t(d) * a.p.row_stride + t * 8;
-                    const bool in = kb + d >= kmin && kb + d < kend;
-#pragma unroll
-                    for (int c = 0; c < KC; ++c) kr[u][r][c] = in ? ld_stream(src + 32 * c) : make_uint4(0, 0, 0, 0);
-                }
-            }
-        };
-        auto load_v = [&](int base, const int64_t (&off)[KT]) {
-#pragma unroll
-            for (int u = 0; u < KT; ++u) {
-                const int kb = base + 16 * u;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 2 * t + (r & 1) + 8 * (r >> 1);
-                    const __nv_bfloat16 *src = V + off[u] + int64_t(d) * a.p.row_stride + g * 8;
-                    const bool in = kb + d >= kmin && kb + d < kend;  // rows outside are never read: they may hold anything
-#pragma unroll
-                    for (int c = 0; c < VC; ++c) vr[u][r][c] = in ? ld_stream(src + 64 * c) : make_uint4(0, 0, 0, 0);
-                }
-            }
-        };
-        int64_t off[KT];
-        int next[KT];
-#pragma unroll
-        for (int u = 0; u < KT; ++u) off[u] = offset(first + 16 * u, page_of(first + 16 * u));
-        load_k(first, off);
-        load_v(first, off);
-#pragma unroll
-        for (int u = 0; u < KT; ++u) next[u] = page_of(first + STEP + 16 * u);
+        // the ring always starts at stage 0: a run leaves no copy in flight
+        int stage = 0;
         for (int base = first; base < kend; base += STEP) {
+            if (!wait_soon(&st.bars[stage], (st.parity >> stage) & 1u)) {
+                // gave up (the device error flag is set): the copies still in flight land, bounded again, before the ring can be
+                // reused or released
+                for (int s = 0, k = base; s < kStages && k < kend; ++s, k += STEP) {
+                    const int x = (stage + s) % kStages;
+                    if (s < kStages - 1) wait_soon(&st.bars[x], (st.parity >> x) & 1u), st.parity ^= 1u << x;
+                }
+                break;
+            }
+            st.parity ^= 1u << stage;
+            {   // the stage before this one has been read by every lane
+                const int free = stage == 0 ? kStages - 1 : stage - 1;
+                __syncwarp();
+                if (lane == 0) fence_proxy_async();
+                issue(base + (kStages - 1) * STEP, free);
+            }
+            const uint32_t in = st.ring + uint32_t(stage) * kStage;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            // chunk c of row r of a box lies at r * 128 + (c ^ (r % 8)) * 16
+            uint4 kr[KT][2][KC];
+#pragma unroll
+            for (int u = 0; u < KT; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) kr[u][r][c] = lds16(in + (u + (c >> 1)) * kBox + (g + 8 * r) * 128 + (((t + 4 * (c & 1)) ^ g) << 4));
             // S^T: keys g and g + 8 (registers 0-1, 2-3) of rows 2 t, 2 t + 1
             float s[KT][NT][4];
 #pragma unroll
             for (int u = 0; u < KT; ++u)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    // independent chains: one a part of q, or one a half of the chunks' words
-                    constexpr int CH = PIECES == 1 ? 2 : PIECES;
+                    // independent chains (a product waits some 35 clocks for the one before it in its chain): one a part of q
+                    // and half of a chunk's words, with bf16 q also one a half of the chunks
+                    constexpr int CH = PIECES == 1 ? 4 : 2 * PIECES;
                     float d[CH][4];
 #pragma unroll
                     for (int y = 0; y < CH; ++y)
@@ -176,18 +226,16 @@ struct MmaCore {
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int p = 0; p < PIECES; ++p)
-                                mma16816(d[PIECES == 1 ? h : p], word(kr[u][0][c], 2 * h), word(kr[u][1][c], 2 * h), word(kr[u][0][c], 2 * h + 1),
-                                         word(kr[u][1][c], 2 * h + 1), q[n][p][c][2 * h], q[n][p][c][2 * h + 1]);
+                                mma16816(d[PIECES == 1 ? 2 * (c & 1) + h : 2 * p + h], word(kr[u][0][c], 2 * h), word(kr[u][1][c], 2 * h),
+                                         word(kr[u][0][c], 2 * h + 1), word(kr[u][1][c], 2 * h + 1), q[n][p][c][2 * h], q[n][p][c][2 * h + 1]);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) s[u][n][x] = PIECES == 1 ? d[0][x] + d[1][x] : (d[CH - 1][x] + d[1][x]) + d[0][x];
+                    for (int x = 0; x < 4; ++x) {
+                        float sum = d[CH - 2][x] + d[CH - 1][x];  // the small parts first
+#pragma unroll
+                        for (int y = CH - 4; y >= 0; y -= 2) sum += d[y][x] + d[y + 1][x];
+                        s[u][n][x] = sum;
+                    }
                 }
-            // the next step's K, and its page after that
-#pragma unroll
-            for (int u = 0; u < KT; ++u) {
-                off[u] = offset(base + STEP + 16 * u, next[u]);
-                next[u] = page_of(base + 2 * STEP + 16 * u);
-            }
-            load_k(base + STEP, off);
             const bool mask = base < all_lo || base + 16 * KT > all_hi;
             bool move = false;
 #pragma unroll
@@ -240,32 +288,61 @@ struct MmaCore {
                         for (int p = 0; p < PIECES; ++p) pf[u][n][p][x] = transpose8x8(w[p]);
                     }
             }
-            // O^T += V^T P^T: elements 8 (g + 8 i) + 2 e (registers 0-1) and + 1 (2-3) of rows 2 t, 2 t + 1
+            uint4 vr[KT][4][VC];
+            const bool cut = base < kmin || base + 16 * KT > kend;  // rows outside the range may hold anything, NaN too
 #pragma unroll
-            for (int i = 0; i < VC; ++i)
+            for (int u = 0; u < KT; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float d[NT][4];
+                for (int r = 0; r < 4; ++r) {
+                    const int d = 2 * t + (r & 1) + 8 * (r >> 1), key = base + 16 * u + d;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) d[n][x] = PIECES == 1 ? acc[i][e][n][x] : 0.f;
-#pragma unroll
-                    for (int u = 0; u < KT; ++u) {
-                        const uint32_t w0 = word(vr[u][0][i], e), w1 = word(vr[u][1][i], e), w2 = word(vr[u][2][i], e), w3 = word(vr[u][3][i], e);
-                        const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
-                        const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int p = PIECES - 1; p >= 0; --p) mma16816(d[n], a0, a1, a2, a3, pf[u][n][p][0], pf[u][n][p][1]);
+                    for (int c = 0; c < VC; ++c) {
+                        vr[u][r][c] = lds16(in + (2 + u + c) * kBox + d * 128 + ((g ^ (d & 7)) << 4));
+                        if (cut && (key < kmin || key >= kend)) vr[u][r][c] = make_uint4(0, 0, 0, 0);
                     }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[i][e][n][x] = PIECES == 1 ? d[n][x] : acc[i][e][n][x] + d[n][x];
                 }
-            load_v(base + STEP, off);
+            // O^T += V^T P^T: elements 8 (g + 8 i) + 2 e (registers 0-1) and + 1 (2-3) of rows 2 t, 2 t + 1; the products of all
+            // elements are independent chains
+            if constexpr (PIECES == 1) {
+#pragma unroll
+                for (int u = 0; u < KT; ++u)
+#pragma unroll
+                    for (int i = 0; i < VC; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t w0 = word(vr[u][0][i], e), w1 = word(vr[u][1][i], e), w2 = word(vr[u][2][i], e), w3 = word(vr[u][3][i], e);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+                                mma16816(acc[i][e][n], __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                                         __byte_perm(w2, w3, 0x7632), pf[u][n][0][0], pf[u][n][0][1]);
+                        }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < VC; ++i) {
+                        float d[4][4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) d[e][x] = 0.f;
+#pragma unroll
+                        for (int u = 0; u < KT; ++u)
+#pragma unroll
+                            for (int p = PIECES - 1; p >= 0; --p)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t w0 = word(vr[u][0][i], e), w1 = word(vr[u][1][i], e), w2 = word(vr[u][2][i], e),
+                                                   w3 = word(vr[u][3][i], e);
+                                    mma16816(d[e], __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                                             __byte_perm(w2, w3, 0x7632), pf[u][n][p][0], pf[u][n][p][1]);
+                                }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) acc[i][e][n][x] += d[e][x];
+                    }
+            }
         }
         // the warps' parts of each row
 #pragma unroll
@@ -300,7 +377,7 @@ int attn_mma_launch(AttnArgs &a, int head_dim, int rows_blk, int dtype, int fram
 }
 int attn_mma_resident(int head_dim, int rows_blk, int dtype) {
     return with_core(head_dim, rows_blk, dtype,
-                     [](auto core) { return resident_blocks((const void *)attn_stream_kernel<decltype(core)>, kRowsThreads, 0); });
+                     [](auto core) { return rows_resident<decltype(core)>(); });
 }
 
 int attn_mma_take_device_error(unsigned int *flags) { return take_device_error(flags); }

@@ -1,8 +1,10 @@
 // The frame around the kernels of few query rows (attn.cu on f32 caches, attn_mma.cu on bf16 caches): which rows and keys a
 // block takes, and where its result goes. A core computes softmax statistics and unnormalised output of up to RB rows over
 // a range of keys, one part a warp, into shared memory:
-//   struct Core { static constexpr int HD, RB, kMinBlocks; using Q = ...;
-//                 static void run(const AttnArgs &, const RowsJob &, float (*acc)[RB][HD], float2 (*ml)[RB]); };
+//   struct Core { static constexpr int HD, RB, kMinBlocks; static constexpr size_t kSmem (dynamic shared memory); using Q = ...;
+//                 struct State (of a thread, through all its jobs); static void init(State &);
+//                 static void run(const AttnArgs &, const RowsJob &, float (*acc)[RB][HD], float2 (*ml)[RB], State &, F between); };
+// (between() is called by every thread while the first copies of the job are on their way.)
 // Three frames use it:
 //   attn_grid_kernel     one block a job of attn_job() (many row tiles, or a prefix); splits meet in attn_merge_kernel.
 //   attn_cluster_kernel  one cluster of blocks a sequence and key/value head: the blocks share its keys evenly and join
@@ -91,14 +93,16 @@ __device__ __forceinline__ void add_prefix(const AttnArgs &a, Join &t, int tok, 
 // ------------------------------------------------------------------ one block a job
 
 template <class Core>
-__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_grid_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_grid_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
     __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
     pdl_enter();
+    typename Core::State core;
+    Core::init(core);
     const AttnJob j = attn_job(a, blockIdx.x);
     for (int row0 = j.tile * RB; row0 < j.rows; row0 += j.tiles * RB) {
-        Core::run(a, RowsJob{j.tok0, j.rows, row0, j.kvh, j.base, j.causal, j.k0, j.k1, j.pages}, s_acc, s_ml);
+        Core::run(a, RowsJob{j.tok0, j.rows, row0, j.kvh, j.base, j.causal, j.k0, j.k1, j.pages}, s_acc, s_ml, core, [] {});
         __syncthreads();
         for (int x = threadIdx.x; x < RB * (HD / 4); x += kRowsThreads) {
             const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
@@ -146,11 +150,13 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
 
 // Grid: clusters of a.cluster blocks; cluster c takes key/value head c % kv_heads of sequence c / kv_heads.
 template <class Core>
-__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
     __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
     pdl_enter();
+    typename Core::State core;
+    Core::init(core);
     const uint32_t rank = cluster_rank(), c = blockIdx.x / uint32_t(a.cluster);
     const uint32_t b = a.kvdiv.div(c);
     const int kvh = int(c - b * uint32_t(a.p.kv_heads));
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_k
     const int k0 = min(lo + int(rank) * per, kv), k1 = min(k0 + per, kv);
     const int32_t *pages = a.p.table + int64_t(b) * a.p.table_stride;
     for (int row0 = 0; row0 < rows; row0 += RB) {  // the same rows in every block of the cluster
-        Core::run(a, RowsJob{tok0, rows, row0, kvh, kv - n, true, k0, k1, pages}, s_acc, s_ml);
+        Core::run(a, RowsJob{tok0, rows, row0, kvh, kv - n, true, k0, k1, pages}, s_acc, s_ml, core, [] {});
         __syncthreads();
         Join mine[(RB * (HD / 4) + kRowsThreads - 1) / kRowsThreads];
 #pragma unroll
@@ -202,120 +208,119 @@ __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_k
 
 // ------------------------------------------------------------------ equal runs of all sequences' key tiles
 
-// Key tiles of sequence b (for one key/value head) and its first key: none for a sequence without new tokens.
+// Key tiles of sequence b (for one key/value head) and its first key: none for a sequence without new tokens. The list's
+// positions fit 31 bits (attn.cu).
 __device__ __forceinline__ int stream_tiles(const AttnArgs &a, int b, int &tok0, int &n, int &kv, int &lo) {
     seq_tokens(a.p, b, tok0, n);
     kv = seq_rows(a.p, b);
     lo = a.window > 0 ? max(kv - n + 1 - a.window, 0) & ~15 : 0;
-    return n > 0 ? (kv - lo + a.stream_keys - 1) / a.stream_keys : 0;
+    return n > 0 ? (kv - lo + (1 << a.stream_shift) - 1) >> a.stream_shift : 0;
 }
-// Block-wide: the number of all tiles of one key/value head, and the sequence whose tiles hold tile `at / kv_heads`-wise
-// position `at` of the list (every sequence's tiles times kv_heads), with the list position of its first tile.
-struct StreamAt {
-    int64_t total;
-    int seq;
-    int64_t start;
+// The list cut into `blocks` runs of `per` tiles, the first `rem` of them one longer.
+struct StreamCut {
+    int blocks, per, rem;
+    __device__ __forceinline__ StreamCut(int total, int grid) {
+        blocks = max(min(total, grid), 1);  // no block without a tile between two that share a sequence
+        per = total / blocks;
+        rem = total - per * blocks;
+    }
+    __device__ __forceinline__ int start(int c) const { return c * per + min(c, rem); }
+    __device__ __forceinline__ int block_of(int u) const {
+        const int x = rem * (per + 1);
+        return u < x ? u / (per + 1) : rem + (u - x) / per;
+    }
 };
-__device__ __forceinline__ int64_t stream_total(const AttnArgs &a, int64_t (&part)[kRowsThreads], int64_t &before, int &b0, int &b1) {
-    const int per = (a.p.seqs + kRowsThreads - 1) / kRowsThreads;
-    b0 = min(int(threadIdx.x) * per, a.p.seqs), b1 = min(b0 + per, a.p.seqs);
-    int64_t sum = 0;
-    for (int b = b0; b < b1; ++b) {
-        int t, n, kv, lo;
-        sum += stream_tiles(a, b, t, n, kv, lo);
-    }
-    sum *= a.p.kv_heads;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    if (lane == 31) part[warp] = inc;
-    __syncthreads();
-    int64_t total = 0;
-    before = inc - sum;
-#pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) {
-        if (w < warp) before += part[w];
-        total += part[w];
-    }
-    return total;
-}
 
-// Where a block stands in the list, kept in shared memory: the registers belong to the core.
+// Where a block stands in the list, and its next job; in shared memory: the registers belong to the core.
 struct StreamState {
-    int64_t u, u1, start, total;  // next tile, end of the block's run, first tile of sequence b, all tiles
-    int b, tiles, extra;
-    RowsJob job;
-    int part;                     // of the workspace; -1: the rows are stored
+    int u, u1, start;  // next tile, end of the block's run, first tile of sequence b
+    int b, extra, tiles;
+    int part[2];       // of the workspace; -1: the rows are stored
+    RowsJob job[2];    // tok0 < 0: no more
 };
+
+// Writes the block's next job into slot `s` (one thread).
+template <int RB>
+__device__ __forceinline__ void stream_next(const AttnArgs &a, StreamState &st, const StreamCut &cut, int s) {
+    const int u = st.u;
+    if (u >= st.u1) {
+        st.job[s].tok0 = -1;
+        return;
+    }
+    int b = st.b, start = st.start, tok0, n, kv, lo;
+    const int extra = st.extra;
+    int tiles = stream_tiles(a, b, tok0, n, kv, lo);
+    while (u >= start + tiles * a.p.kv_heads) {
+        start += tiles * a.p.kv_heads;
+        tiles = stream_tiles(a, ++b, tok0, n, kv, lo);
+    }
+    const int kvh = (u - start) / tiles;
+    const int s0 = start + kvh * tiles;  // the list positions of this sequence and head: s0 .. s0 + tiles
+    const int e = min(s0 + tiles, st.u1);
+    const bool head = u == s0, whole = head && e == s0 + tiles;
+    const int rows = n * a.p.group;
+    // rows past RB (a sequence with more new tokens than the host's bound): the block of the first tile takes them over all
+    // keys
+    st.job[s] = RowsJob{tok0, rows, extra * RB, kvh, kv - n, true, extra ? lo : min(lo + ((u - s0) << a.stream_shift), kv),
+                        extra ? kv : min(lo + ((e - s0) << a.stream_shift), kv), a.p.table + int64_t(b) * a.p.table_stride};
+    st.part[s] = (whole && a.pre_splits == 0) || extra ? -1 : whole ? 2 * a.stream_blocks + b * a.p.kv_heads + kvh : 2 * int(blockIdx.x) + (head ? 1 : 0);
+    if (head) a.stream_desc[int64_t(b) * a.p.kv_heads + kvh] = make_int2(int(blockIdx.x), whole ? int(blockIdx.x) : cut.block_of(s0 + tiles - 1));
+    const bool more = head && (extra + 1) * RB < rows;
+    st.extra = more ? extra + 1 : 0;
+    st.u = more ? u : e;
+    st.start = start, st.b = b;
+}
 
 template <class Core>
-__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
     __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
-    __shared__ int64_t s_part[kRowsThreads];
+    __shared__ int s_part[kRowsWarps];
     __shared__ StreamState st;
     pdl_enter();
-    {
-        int64_t before;
-        int b0, b1;
-        const int64_t c = blockIdx.x, total = stream_total(a, s_part, before, b0, b1);
-        const int64_t blocks = min(int64_t(gridDim.x), total);  // no block without a tile between two that share a sequence
-        if (c >= blocks) return;
-        const int64_t u = total * c / blocks;
-        if (threadIdx.x == 0) st.u = u, st.u1 = total * (c + 1) / blocks, st.total = total, st.extra = 0;
-        for (int x = b0; x < b1; ++x) {  // the thread whose sequences hold tile u
-            int t, n, kv, lo;
-            const int tiles = stream_tiles(a, x, t, n, kv, lo);
-            const int64_t w = int64_t(tiles) * a.p.kv_heads;
-            if (u >= before && u < before + w) st.b = x, st.start = before, st.tiles = tiles;
-            before += w;
+    typename Core::State core;
+    Core::init(core);
+    int total;
+    {   // all tiles, and the sequence that holds the block's first: every thread sums a run of sequences, then a prefix sum
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int per = (a.p.seqs + kRowsThreads - 1) / kRowsThreads;
+        const int b0 = min(int(threadIdx.x) * per, a.p.seqs), b1 = min(b0 + per, a.p.seqs);
+        int t, n, kv, lo, sum = 0;
+        for (int x = b0; x < b1; ++x) sum += stream_tiles(a, x, t, n, kv, lo);
+        sum *= a.p.kv_heads;
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
         }
+        if (lane == 31) s_part[warp] = inc;
         __syncthreads();
+        int before = inc - sum;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) {
+            if (w < warp) before += s_part[w];
+            total += s_part[w];
+        }
+        const StreamCut cut(total, int(gridDim.x));
+        if (total == 0 || int(blockIdx.x) >= cut.blocks) return;
+        const int u = cut.start(int(blockIdx.x));
+        if (u >= before && u < before + sum) {  // this thread's sequences hold it
+            st.u = u, st.u1 = cut.start(int(blockIdx.x) + 1), st.extra = 0, st.b = b0, st.start = before;
+            stream_next<RB>(a, st, cut, 0);
+        }
     }
-    for (;;) {
-        if (threadIdx.x == 0) {
-            int64_t u = st.u, start = st.start;
-            int b = st.b, tiles = st.tiles, tok0, n, kv, lo;
-            const int extra = st.extra;
-            if (u < st.u1) {
-                tiles = stream_tiles(a, b, tok0, n, kv, lo);
-                while (u >= start + int64_t(tiles) * a.p.kv_heads) {
-                    start += int64_t(tiles) * a.p.kv_heads;
-                    tiles = stream_tiles(a, ++b, tok0, n, kv, lo);
-                }
-                const int kvh = int((u - start) / tiles);
-                const int64_t s0 = start + int64_t(kvh) * tiles;  // the list positions of this sequence and head: s0 .. s0 + tiles
-                const int64_t e = min(s0 + tiles, st.u1);
-                const bool head = u == s0, whole = head && e == s0 + tiles;
-                const int rows = n * a.p.group;
-                // rows past RB (a sequence with more new tokens than the host's bound): the block of the first tile takes them
-                // over all keys
-                st.job = RowsJob{tok0, rows, extra * RB, kvh, kv - n, true, extra ? lo : min(lo + int(u - s0) * a.stream_keys, kv),
-                                 extra ? kv : min(lo + int(e - s0) * a.stream_keys, kv), a.p.table + int64_t(b) * a.p.table_stride};
-                st.part = (whole && a.pre_splits == 0) || extra ? -1 : whole ? 2 * a.stream_blocks + b * a.p.kv_heads + kvh : 2 * int(blockIdx.x) + (head ? 1 : 0);
-                // the blocks that share this sequence and head: block of tile u is the c with total c / blocks <= u < total (c + 1)
-                // / blocks (rounded down)
-                const int64_t blocks = min(int64_t(gridDim.x), st.total);
-                if (head) a.stream_desc[int64_t(b) * a.p.kv_heads + kvh] = make_int2(int(blockIdx.x), int(((s0 + tiles) * blocks - 1) / st.total));
-                const bool more = head && (extra + 1) * RB < rows;
-                st.extra = more ? extra + 1 : 0;
-                st.u = more ? u : e;
-                st.start = start, st.b = b, st.tiles = tiles;
-            } else {
-                st.job.tok0 = -1;
-            }
-        }
+    for (int s = 0;; s ^= 1) {
         __syncthreads();
-        if (st.job.tok0 < 0) return;
-        Core::run(a, st.job, s_acc, s_ml);
+        if (st.job[s].tok0 < 0) return;
+        Core::run(a, st.job[s], s_acc, s_ml, core, [&] {
+            if (threadIdx.x == 0) stream_next<RB>(a, st, StreamCut(total, int(gridDim.x)), s ^ 1);
+        });
         __syncthreads();
-        const RowsJob j = st.job;
-        const int64_t part = st.part;
+        const RowsJob j = st.job[s];
+        const int64_t part = st.part[s];
         for (int x = threadIdx.x; x < RB * (HD / 4); x += kRowsThreads) {
             const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
             if (j.row0 + r >= j.rows) break;
@@ -335,7 +340,6 @@ __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_ke
             }
             store4(static_cast<typename Core::Q *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
         }
-        __syncthreads();
     }
 }
 
@@ -426,11 +430,42 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const A
 
 // ------------------------------------------------------------------ launches
 
+// Allows a kernel its dynamic shared memory, once a device.
+template <class Core>
+bool rows_allow(const void *kern, uint64_t &done) {
+    if (Core::kSmem <= 48 * 1024) return true;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Core::kSmem)) != cudaSuccess) return false;
+    __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+    return true;
+}
+template <class Core>
+bool rows_ready(int frame) {
+    static uint64_t done[3] = {};
+    return frame == kFrameCluster  ? rows_allow<Core>((const void *)attn_cluster_kernel<Core>, done[frame])
+           : frame == kFrameStream ? rows_allow<Core>((const void *)attn_stream_kernel<Core>, done[frame])
+                                   : rows_allow<Core>((const void *)attn_grid_kernel<Core>, done[frame]);
+}
+// Blocks of the stream frame on the device at once.
+template <class Core>
+int rows_resident() {
+    if (!rows_ready<Core>(kFrameStream)) {
+        cudaGetLastError();  // without a device (a size query): what the launch will find
+        return sm_count();
+    }
+    return resident_blocks((const void *)attn_stream_kernel<Core>, kRowsThreads, Core::kSmem);
+}
+
 // Launches the frame that the shape asks for (attn.cu): blocks of the grid or stream kernel, or clusters.
 template <class Core>
 int launch_rows(AttnArgs &a, int frame, int64_t units, cudaStream_t st, const char *name) {
+    if (!rows_ready<Core>(frame)) return check_launch(name);
     if (frame == kFrameCluster) {
         cudaLaunchConfig_t cfg = {};
+        cfg.dynamicSmemBytes = Core::kSmem;
         cfg.gridDim = dim3(unsigned(units * a.cluster));
         cfg.blockDim = kRowsThreads;
         cfg.stream = st;
@@ -443,11 +478,11 @@ int launch_rows(AttnArgs &a, int frame, int64_t units, cudaStream_t st, const ch
         cfg.numAttrs = pdl_enabled() ? 2 : 1;
         cudaLaunchKernelEx(&cfg, attn_cluster_kernel<Core>, a);
     } else if (frame == kFrameStream) {
-        launch_k(attn_stream_kernel<Core>, dim3(unsigned(units)), kRowsThreads, 0, st, a);
+        launch_k(attn_stream_kernel<Core>, dim3(unsigned(units)), kRowsThreads, Core::kSmem, st, a);
         launch_k(attn_stream_merge_kernel<typename Core::Q, Core::HD>, dim3(unsigned(a.stream_rows * a.p.kv_heads * a.p.seqs)), kRowsThreads, 0, st,
                  a);
     } else {
-        launch_k(attn_grid_kernel<Core>, dim3(unsigned(units)), kRowsThreads, 0, st, a);
+        launch_k(attn_grid_kernel<Core>, dim3(unsigned(units)), kRowsThreads, Core::kSmem, st, a);
     }
     return check_launch(name);
 }

@@ -74,22 +74,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// Bounded wait of a converged warp, as mbar_wait_warp, in little code whose first 256 polls touch neither the timer nor
-// memory: the waits of this kernel last a few hundred clocks, and its warps share their instruction caches.
-__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity) {
-    uint64_t t0 = 0;
-#pragma unroll 1
-    for (uint32_t i = 1;; ++i) {
-        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-        if ((i & 255u) == 0) {
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            if (__any_sync(0xffffffffu, now - t0 > kWaitLimitNs)) break;
-        }
-    }
-    if ((threadIdx.x & 31) == 0) atomicOr(&g_device_error, kDevErrTimeout);
-    return false;
-}
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
@@ -110,13 +94,6 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     return mul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3F800000u),
                                __uint_as_float((__float_as_uint(t.y) << 23) + 0x3F800000u)));
 }
-// Tiled tensor copy of a 4-D map's box; x times the element size is a multiple of 128 bytes at every call site.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
-                 : "memory");
-}
-
 struct TcJob {
     int ok;
     int tok0, rows, row0;  // tokens of the job start at tok0; this block's rows row0 .. of `rows`
@@ -537,23 +514,6 @@ PFN_cuTensorMapEncodeTiled_v12000 encode() {
     return fn;
 }
 
-// Map of one of the cache's tensors: [pages][page rows][kv heads][hd], box 64 elements of one head x up to 128 rows of one
-// page, 128-byte swizzle.
-int cache_map(const vox_cuda_kv_cache &c, const void *base, CUtensorMap &m, const std::string &name) {
-    auto fn = encode();
-    if (!fn) return set_error(VOX_CUDA_ERR_DEVICE, name + ": cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.kv_heads), cuuint64_t(c.page_size), cuuint64_t(c.pages)};
-    // a dimension of one element is never stepped: any stride that the encoder accepts
-    const int64_t page = c.pages > 1 ? c.page_stride : c.row_stride * c.page_size, head = c.kv_heads > 1 ? c.head_stride : c.head_dim;
-    const cuuint64_t strides[3] = {cuuint64_t(head) * 2, cuuint64_t(c.row_stride) * 2, cuuint64_t(page) * 2};
-    const cuuint32_t box[4] = {64, 1, cuuint32_t(c.page_size < kKeys ? c.page_size : kKeys), 1};
-    const cuuint32_t es[4] = {1, 1, 1, 1};
-    const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return set_error(VOX_CUDA_ERR_ARG, name + ": cache tensor map rejected (code " + std::to_string(int(r)) + ")");
-    return VOX_CUDA_OK;
-}
-
 template <int HD>
 int launch(const AttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int64_t blocks, cudaStream_t st, const char *name) {
     auto kern = attn_tc_kernel<HD>;
@@ -570,10 +530,26 @@ int launch(const AttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int6
 
 }  // namespace
 
+int attn_cache_map(const vox_cuda_kv_cache &c, const void *base, int box_rows, CUtensorMap &m, const char *name) {
+    auto fn = encode();
+    if (!fn) return set_error(VOX_CUDA_ERR_DEVICE, std::string(name) + ": cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.kv_heads), cuuint64_t(c.page_size), cuuint64_t(c.pages)};
+    // a dimension of one element is never stepped: any stride that the encoder accepts
+    const int64_t page = c.pages > 1 ? c.page_stride : c.row_stride * c.page_size, head = c.kv_heads > 1 ? c.head_stride : c.head_dim;
+    const cuuint64_t strides[3] = {cuuint64_t(head) * 2, cuuint64_t(c.row_stride) * 2, cuuint64_t(page) * 2};
+    const cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(VOX_CUDA_ERR_ARG, std::string(name) + ": cache tensor map rejected (code " + std::to_string(int(r)) + ")");
+    return VOX_CUDA_OK;
+}
+
 int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name) {
     CUtensorMap mk, mv;
-    int rc = cache_map(c, c.k, mk, name);
-    if (rc == VOX_CUDA_OK) rc = cache_map(c, c.v, mv, name);
+    const int rows = c.page_size < kKeys ? c.page_size : kKeys;  // a box never leaves a page
+    int rc = attn_cache_map(c, c.k, rows, mk, name);
+    if (rc == VOX_CUDA_OK) rc = attn_cache_map(c, c.v, rows, mv, name);
     if (rc != VOX_CUDA_OK) return rc;
     return c.head_dim == 64 ? launch<64>(a, mk, mv, blocks, st, name) : launch<128>(a, mk, mv, blocks, st, name);
 }

@@ -27,7 +27,7 @@ struct AttnArgs {
     int32_t own_splits, own_chunk, own_tiles;  // tiles: blocks over the rows of a sequence
     // the prefix: likewise, over the rows of all tokens
     int32_t pre_splits, pre_chunk, pre_tiles;
-    FastDiv kvdiv, otdiv, osdiv, ptdiv;        // divisions by kv_heads, own_tiles, own_splits, pre_tiles
+    FastDiv kvdiv, otdiv, osdiv, ptdiv, srdiv; // divisions by kv_heads, own_tiles, own_splits, pre_tiles, stream_rows
     int32_t pre_blocks, splits;                // blocks of the prefix (they come first); slots of a row in the workspace
     int32_t partial;                           // results go to the workspace (a row's parts meet in a later launch)
     // the tensor-core kernel: rows a block; whether this launch takes the prefix; whether the own keys follow the prefix

@@ -62,12 +62,17 @@ struct MmaCore {
     struct State {
         uint32_t ring, parity;
         uint64_t *bars;
+        uint8_t *base;
     };
+    // The warps' results take the place of the rings, which hold nothing any more by then.
+    static_assert(size_t(kRowsWarps) * RB * HD_ * 4 <= size_t(kRowsWarps) * kStages * kStage, "results fit the rings");
+    static __device__ __forceinline__ float (*acc(State &st))[RB][HD] { return reinterpret_cast<float(*)[RB][HD]>(st.base); }
     static __device__ __forceinline__ void init(State &st) {
         extern __shared__ uint8_t ring_raw[];
         __shared__ uint64_t s_bars[kRowsWarps][kStages];
         const int warp = threadIdx.x >> 5;
-        st.ring = ((smem_addr(ring_raw) + 1023u) & ~1023u) + uint32_t(warp) * kStages * kStage;
+        st.base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ring_raw) + 1023) & ~uintptr_t(1023));
+        st.ring = smem_addr(st.base) + uint32_t(warp) * kStages * kStage;
         st.bars = s_bars[warp];
         st.parity = 0;
         if ((threadIdx.x & 31) == 0) {
@@ -344,6 +349,7 @@ struct MmaCore {
                     }
             }
         }
+        __syncthreads();  // every warp has read its ring
         // the warps' parts of each row
 #pragma unroll
         for (int n = 0; n < NT; ++n)

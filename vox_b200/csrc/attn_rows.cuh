@@ -2,7 +2,7 @@
 // block takes, and where its result goes. A core computes softmax statistics and unnormalised output of up to RB rows over
 // a range of keys, one part a warp, into shared memory:
 //   struct Core { static constexpr int HD, RB, kMinBlocks; static constexpr size_t kSmem (dynamic shared memory); using Q = ...;
-//                 struct State (of a thread, through all its jobs); static void init(State &);
+//                 struct State (of a thread, through all its jobs); static void init(State &); static (*acc(State &))[RB][HD];
 //                 static void run(const AttnArgs &, const RowsJob &, float (*acc)[RB][HD], float2 (*ml)[RB], State &, F between); };
 // (between() is called by every thread while the first copies of the job are on their way.)
 // Three frames use it:
@@ -95,11 +95,11 @@ __device__ __forceinline__ void add_prefix(const AttnArgs &a, Join &t, int tok, 
 template <class Core>
 __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_grid_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
-    __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
     pdl_enter();
     typename Core::State core;
     Core::init(core);
+    float(*s_acc)[RB][HD] = Core::acc(core);
     const AttnJob j = attn_job(a, blockIdx.x);
     for (int row0 = j.tile * RB; row0 < j.rows; row0 += j.tiles * RB) {
         Core::run(a, RowsJob{j.tok0, j.rows, row0, j.kvh, j.base, j.causal, j.k0, j.k1, j.pages}, s_acc, s_ml, core, [] {});
@@ -152,11 +152,11 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
 template <class Core>
 __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
-    __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
     pdl_enter();
     typename Core::State core;
     Core::init(core);
+    float(*s_acc)[RB][HD] = Core::acc(core);
     const uint32_t rank = cluster_rank(), c = blockIdx.x / uint32_t(a.cluster);
     const uint32_t b = a.kvdiv.div(c);
     const int kvh = int(c - b * uint32_t(a.p.kv_heads));
@@ -274,13 +274,13 @@ __device__ __forceinline__ void stream_next(const AttnArgs &a, StreamState &st, 
 template <class Core>
 __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
-    __shared__ float s_acc[kRowsWarps][RB][HD];
     __shared__ float2 s_ml[kRowsWarps][RB];
     __shared__ int s_part[kRowsWarps];
     __shared__ StreamState st;
     pdl_enter();
     typename Core::State core;
     Core::init(core);
+    float(*s_acc)[RB][HD] = Core::acc(core);
     int total;
     {   // all tiles, and the sequence that holds the block's first: every thread sums a run of sequences, then a prefix sum
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -343,19 +343,21 @@ __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_ke
     }
 }
 
-// One block a sequence and query-head row: joins the parts of the shared prefix and of the blocks that share the
-// sequence's keys; rows that one block took whole are stored already (without a prefix). Warp w takes parts w, w + 4, ..,
-// lane: elements E lane .. of the row. Grid: (rows of a sequence up to RB) * kv_heads * seqs.
-template <typename QT, int HD>
-__global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const AttnArgs a) {
-    constexpr int E = HD / 32;
+// Joins, for each sequence and query-head row, the parts of the shared prefix and of the blocks that share the sequence's
+// keys; rows that one block took whole are stored already (without a prefix). WPR warps a row (one where there are rows
+// enough for the device, four where there are few): warp w of them takes parts w, w + WPR, .., lane: elements E lane .. of
+// the row. Rows: (rows of a sequence up to RB) * kv_heads * seqs.
+template <typename QT, int HD, int WPR>
+__global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int E = HD / 32, RPB = kRowsWarps / WPR;
     __shared__ __align__(16) float s_o[kRowsWarps][HD];
     __shared__ float2 s_ml[kRowsWarps];
     pdl_enter();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int r = int(blockIdx.x % uint32_t(a.stream_rows));
-    const uint32_t y = blockIdx.x / uint32_t(a.stream_rows), b = a.kvdiv.div(y);
-    const int kvh = int(y - b * uint32_t(a.p.kv_heads));
+    const int warp = (threadIdx.x >> 5) % WPR, lane = threadIdx.x & 31;
+    const uint32_t id = blockIdx.x * RPB + (threadIdx.x >> 5) / WPR;
+    const uint32_t y = a.srdiv.div(id), b = a.kvdiv.div(y);
+    const int r = int(id - y * uint32_t(a.stream_rows)), kvh = int(y - b * uint32_t(a.p.kv_heads));
+    if (int(b) >= a.p.seqs) return;  // the whole row's warps (WPR 4: the whole block)
     const int2 desc = __ldcg(a.stream_desc + y);
     int tok0, n, kv, lo;
     const int tiles = stream_tiles(a, int(b), tok0, n, kv, lo);
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const A
         int tok, h;
         row_of(a, tok0, kvh, row, tok, h);
         const int64_t pre = (int64_t(tok) * a.p.heads + h) * a.splits;
-        const int parts = a.pre_splits + own, mine = (parts - warp + kRowsWarps - 1) / kRowsWarps;
+        const int parts = a.pre_splits + own, mine = (parts - warp + WPR - 1) / WPR;
         // part p: a slot of the prefix, or the c0-th, .. block's part of the own keys (kept as a whole where there is one)
         auto slot = [&](int p, const float2 *&ml, const float *&o) {
             if (p < a.pre_splits) {
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const A
             const int cnt = min(mine - base, 32);
             const float2 *ml;
             const float *po;
-            slot(warp + (base + min(lane, cnt - 1)) * kRowsWarps, ml, po);
+            slot(warp + (base + min(lane, cnt - 1)) * WPR, ml, po);
             const float2 v = lane < cnt ? __ldcg(ml) : make_float2(-INFINITY, 0.f);
             const float mx = fmaxf(m, warp_max(v.x)), ms = mx == -INFINITY ? 0.f : mx;
             const float alpha = ex2_approx(m - ms), w = ex2_approx(v.x - ms);
@@ -397,16 +399,22 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const A
             l = l * alpha + warp_sum(v.x == -INFINITY ? v.y : v.y * w);
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] *= alpha;
-            for (int k = 0; k < cnt; k += 4) {  // four parts in flight
-                float x[4][E];
+            constexpr int U = 8;  // parts in flight
+            for (int k = 0; k < cnt; k += U) {
+                float x[U][E];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(po), min(k + u, cnt - 1)));
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[u][e] = __ldcg(src + lane * E + e);
+                for (int u = 0; u < U; ++u) {
+                    const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(po), min(k + u, cnt - 1))) + lane * E;
+                    if constexpr (E == 4) {
+                        const float4 f = __ldcg(reinterpret_cast<const float4 *>(src));
+                        x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
+                    } else {
+                        const float2 f = __ldcg(reinterpret_cast<const float2 *>(src));
+                        x[u][0] = f.x, x[u][1] = f.y;
+                    }
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < U; ++u) {
                     const float wu = __shfl_sync(0xffffffffu, w, min(k + u, 31));
                     if (k + u < cnt)
 #pragma unroll
@@ -414,17 +422,28 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const A
                 }
             }
         }
+        QT *dst = static_cast<QT *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD;
+        if constexpr (WPR == 1) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            if constexpr (E == 4)
+                store4(dst + lane * E, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
+            else if constexpr (sizeof(QT) == 4)
+                *reinterpret_cast<float2 *>(dst + lane * E) = make_float2(o[0] * inv, o[1] * inv);
+            else
+                *reinterpret_cast<uint32_t *>(dst + lane * E) = pack_bf16(o[0] * inv, o[1] * inv);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-        if (lane == 0) s_ml[warp] = make_float2(m, l);
-        __syncthreads();
-        for (int d = threadIdx.x * 4; d < HD; d += kRowsThreads * 4) {
-            Join t;
+            for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+            if (lane == 0) s_ml[warp] = make_float2(m, l);
+            __syncthreads();
+            for (int d = threadIdx.x * 4; d < HD; d += kRowsThreads * 4) {
+                Join t;
 #pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) t.add(s_ml[w].x, s_ml[w].y, *reinterpret_cast<const float4 *>(&s_o[w][d]));
-            store4(static_cast<QT *>(a.out) + int64_t(tok) * a.out_stride + int64_t(h) * HD + d, t.out());
+                for (int w = 0; w < kRowsWarps; ++w) t.add(s_ml[w].x, s_ml[w].y, *reinterpret_cast<const float4 *>(&s_o[w][d]));
+                store4(dst + d, t.out());
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -479,8 +498,11 @@ int launch_rows(AttnArgs &a, int frame, int64_t units, cudaStream_t st, const ch
         cudaLaunchKernelEx(&cfg, attn_cluster_kernel<Core>, a);
     } else if (frame == kFrameStream) {
         launch_k(attn_stream_kernel<Core>, dim3(unsigned(units)), kRowsThreads, Core::kSmem, st, a);
-        launch_k(attn_stream_merge_kernel<typename Core::Q, Core::HD>, dim3(unsigned(a.stream_rows * a.p.kv_heads * a.p.seqs)), kRowsThreads, 0, st,
-                 a);
+        const int64_t rows = int64_t(a.stream_rows) * a.p.kv_heads * a.p.seqs;
+        if (rows >= int64_t(sm_count()) * 4)
+            launch_k(attn_stream_merge_kernel<typename Core::Q, Core::HD, 1>, dim3(unsigned((rows + kRowsWarps - 1) / kRowsWarps)), kRowsThreads, 0, st, a);
+        else
+            launch_k(attn_stream_merge_kernel<typename Core::Q, Core::HD, 4>, dim3(unsigned(rows)), kRowsThreads, 0, st, a);
     } else {
         launch_k(attn_grid_kernel<Core>, dim3(unsigned(units)), kRowsThreads, Core::kSmem, st, a);
     }

@@ -193,6 +193,7 @@ int ceil_div(int64_t x, int64_t y) { return int((x + y - 1) / y); }
 // How a call is cut: which kernels take its parts, rows a block, row tiles, key splits.
 struct AttnShape {
     bool own_tc, pre_tc, concat, mma;  // mma: what the tensor-core kernel does not take goes to attn_mma.cu, else to the CUDA cores
+    bool wide, pre_wide;               // or, many rows at f32 accuracy, to attn_f32.cu (the prefix alone, in a launch of its own)
     int frame;                         // of the own keys, where the tensor-core kernel does not take them
     int rows_blk, tc_rows;
     int own_tiles, own_splits, own_chunk;
@@ -217,11 +218,14 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
     const bool f32 = dtype == VOX_CUDA_F32, tc_types = !f32 && bf16_cache;
     s.mma = bf16_cache;
     s.rows_blk = s.mma ? (rows <= 8 || f32 ? 8 : 16) : rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    s.wide = !tc_types && rows > 16;
+    if (s.wide) s.rows_blk = kF32Rows;
+    s.pre_wide = !tc_types && !s.wide && all >= 2 * kF32Rows;
     s.own_tc = tc_types && rows > 16;
     s.pre_tc = tc_types && all > 16;
     s.concat = prefix_len > 0 && s.own_tc && rows >= 64;
     if (prefix_len > 0 && !s.concat) {
-        const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.rows_blk;
+        const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.pre_wide ? kF32Rows : s.rows_blk;
         if (s.pre_tc) s.tc_rows = rb;
         s.pre_tiles = ceil_div(all, rb);
         const int64_t pre = int64_t(p.kv_heads) * s.pre_tiles;
@@ -236,7 +240,7 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         const int64_t own = int64_t(s.own_tiles) * p.kv_heads;
         cut_keys(max_kv, s.concat ? 1 : own < sms ? sms / own : 1, s.own_splits, s.own_chunk);
         s.own_units = own * s.own_splits;
-    } else if (rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc) && base * ((int64_t(p.cap) >> 6) + 1) < (int64_t(1) << 31)) {
+    } else if (!s.wide && rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc || s.pre_wide) && base * ((int64_t(p.cap) >> 6) + 1) < (int64_t(1) << 31)) {
         // one row tile a sequence: a cluster for each sequence and key/value head where one wave of blocks holds them all
         // with at most 512 keys each, else equal runs of all sequences' tiles
         const int64_t resident = s.mma ? attn_mma_resident(head_dim, s.rows_blk, dtype)
@@ -351,12 +355,19 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
         a.tc_prefix = 0;
         if (r != VOX_CUDA_OK) return r;
     }
+    if (s.pre_blocks > 0 && s.pre_wide) {
+        a.pre_blocks = int32_t(s.pre_blocks);
+        r = attn_f32_launch(a, hd, dtype, cache->dtype, s.pre_blocks, st, name);
+        if (r != VOX_CUDA_OK) return r;
+    }
     if (s.own_tc) {
         r = attn_tc_launch(a, *cache, s.own_units, st, name);
     } else {
-        a.pre_blocks = s.pre_tc ? 0 : int32_t(s.pre_blocks);
+        a.pre_blocks = s.pre_tc || s.pre_wide ? 0 : int32_t(s.pre_blocks);
         const int64_t n = a.pre_blocks + s.own_units;
-        if (s.mma) {
+        if (s.wide) {
+            r = attn_f32_launch(a, hd, dtype, cache->dtype, n, st, name);
+        } else if (s.mma) {
             r = attn_cache_map(*cache, cache->k, 16, a.mk, name);
             if (r == VOX_CUDA_OK) r = attn_cache_map(*cache, cache->v, 16, a.mv, name);
             if (r != VOX_CUDA_OK) return r;

@@ -82,7 +82,7 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
     uint32_t y = a.kvdiv.div(x);
     j.kvh = int(x - y * uint32_t(a.p.kv_heads));
     uint32_t z = a.otdiv.div(y);
-    j.tile = int(y - z * uint32_t(a.own_tiles));
+    j.tile = a.own_tiles - 1 - int(y - z * uint32_t(a.own_tiles));  // the last rows, which see most keys, first
     j.tiles = a.own_tiles;
     const uint32_t b = a.osdiv.div(z);
     const int s = int(z - b * uint32_t(a.own_splits));
@@ -104,6 +104,9 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
 // Few rows on a bf16 cache (attn_mma.cu): rows_blk 8, or 16 (bf16 activations); units: blocks, or clusters.
 int attn_mma_launch(AttnArgs &a, int head_dim, int rows_blk, int dtype, int frame, int64_t units, cudaStream_t st, const char *name);
 int attn_mma_resident(int head_dim, int rows_blk, int dtype);  // blocks of the stream frame on the device at once
+// Many rows at f32 accuracy (attn_f32.cu): 64 rows a block, jobs of attn_job().
+constexpr int kF32Rows = 64;
+int attn_f32_launch(const AttnArgs &a, int head_dim, int dtype, int cache_dtype, int64_t blocks, cudaStream_t st, const char *name);
 // Map of one of the cache's tensors: [pages][page rows][kv heads][hd], box 64 elements of one head x box_rows rows of one
 // page, 128-byte swizzle (attn_tc.cu).
 int attn_cache_map(const vox_cuda_kv_cache &c, const void *base, int box_rows, CUtensorMap &m, const char *name);

@@ -848,7 +848,7 @@ extern "C" int vox_cuda_device_error(unsigned int *flags) {
     if (take_device_error(&v) != VOX_CUDA_OK || gemv_take_device_error(&v) != VOX_CUDA_OK || f5_take_device_error(&v) != VOX_CUDA_OK ||
         gemm_take_device_error(&v) != VOX_CUDA_OK || kv_append_take_device_error(&v) != VOX_CUDA_OK ||
         attn_take_device_error(&v) != VOX_CUDA_OK || attn_tc_take_device_error(&v) != VOX_CUDA_OK ||
-        attn_mma_take_device_error(&v) != VOX_CUDA_OK) {
+        attn_mma_take_device_error(&v) != VOX_CUDA_OK || attn_f32_take_device_error(&v) != VOX_CUDA_OK) {
         const cudaError_t e = cudaGetLastError();
         return set_error(VOX_CUDA_ERR_DEVICE, std::string("vox_cuda_device_error: ") + cudaGetErrorString(e));
     }

@@ -54,10 +54,11 @@ int launch_softmax_pipe(const float *x, float *y, int64_t rows, int64_t n, float
 int gemv_take_device_error(unsigned int *flags);
 // The same for the F5 step's attention kernel (f5.cu).
 int f5_take_device_error(unsigned int *flags);
-// And for the paged-cache operators (kv_append.cu, attn.cu, attn_tc.cu, attn_mma.cu).
+// And for the paged-cache operators (kv_append.cu, attn.cu, attn_tc.cu, attn_mma.cu, attn_f32.cu).
 int kv_append_take_device_error(unsigned int *flags);
 int attn_take_device_error(unsigned int *flags);
 int attn_tc_take_device_error(unsigned int *flags);
 int attn_mma_take_device_error(unsigned int *flags);
+int attn_f32_take_device_error(unsigned int *flags);
 
 }  // namespace voxcuda

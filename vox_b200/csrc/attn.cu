@@ -334,7 +334,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.own_splits = s.own_splits, a.own_chunk = s.own_chunk, a.own_tiles = s.own_tiles;
     a.pre_splits = s.pre_splits, a.pre_chunk = s.pre_chunk, a.pre_tiles = s.pre_tiles;
     auto div_by = [](int d) { return FastDiv(uint32_t(d > 0 ? d : 1)); };
-    a.kvdiv = div_by(a.p.kv_heads), a.otdiv = div_by(s.own_tiles), a.osdiv = div_by(s.own_splits), a.ptdiv = div_by(s.pre_tiles), a.srdiv = div_by(s.stream_rows);
+    a.kvdiv = div_by(a.p.kv_heads), a.otdiv = div_by(a.p.seqs * (s.own_splits > 0 ? s.own_splits : 1)), a.osdiv = div_by(s.own_splits), a.ptdiv = div_by(s.pre_tiles), a.srdiv = div_by(s.stream_rows);
     a.splits = s.slots, a.partial = w.partial;
     a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
     a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;

@@ -27,7 +27,7 @@ struct AttnArgs {
     int32_t own_splits, own_chunk, own_tiles;  // tiles: blocks over the rows of a sequence
     // the prefix: likewise, over the rows of all tokens
     int32_t pre_splits, pre_chunk, pre_tiles;
-    FastDiv kvdiv, otdiv, osdiv, ptdiv, srdiv; // divisions by kv_heads, own_tiles, own_splits, pre_tiles, stream_rows
+    FastDiv kvdiv, otdiv, osdiv, ptdiv, srdiv; // divisions by kv_heads, seqs * own_splits, own_splits, pre_tiles, stream_rows
     int32_t pre_blocks, splits;                // blocks of the prefix (they come first); slots of a row in the workspace
     int32_t partial;                           // results go to the workspace (a row's parts meet in a later launch)
     // the tensor-core kernel: rows a block; whether this launch takes the prefix; whether the own keys follow the prefix
@@ -78,11 +78,12 @@ __device__ __forceinline__ AttnJob attn_job(const AttnArgs &a, uint32_t blk) {
         j.k1 = j.split + 1 == a.pre_splits ? a.prefix_len : min(j.k0 + a.pre_chunk, a.prefix_len);
         return j;
     }
+    // row tiles in descending order over all sequences: the last rows, which see most keys, first
     x -= uint32_t(a.pre_blocks);
-    uint32_t y = a.kvdiv.div(x);
+    const uint32_t y = a.kvdiv.div(x);
     j.kvh = int(x - y * uint32_t(a.p.kv_heads));
-    uint32_t z = a.otdiv.div(y);
-    j.tile = a.own_tiles - 1 - int(y - z * uint32_t(a.own_tiles));  // the last rows, which see most keys, first
+    const uint32_t t = a.otdiv.div(y), z = y - t * a.otdiv.d;
+    j.tile = a.own_tiles - 1 - int(t);
     j.tiles = a.own_tiles;
     const uint32_t b = a.osdiv.div(z);
     const int s = int(z - b * uint32_t(a.own_splits));

@@ -7,10 +7,13 @@
 // f32 for every type; a bf16 destination is rounded once, at the store.
 //
 // Bound by HBM at prompts (each projection element is read once and written once, nothing else but a row of the table a
-// token) and by latency at single tokens. Layout: a lane holds one 16-byte vector of a head (4 f32 or 8 bf16), so a head
-// of width hd takes hd / V lanes and the rotation partner p + hd/2 sits in the lane half of them away: one shuffle, no
-// shared memory. A warp takes L such loads of one token, all in flight before the first is used; the token's sequence,
-// length and page are looked up while they fly.
+// token) and by latency at single tokens. Layout: a lane holds a 16-byte vector of a head's first half and the one hd/2
+// further on, the rotation's partners, so the rotation stays in the lane and a head of width hd takes hd / 2V lanes (V = 4
+// f32 or 8 bf16); only the mean square crosses lanes. (One vector a lane, the partner fetched by shuffles: 61 us at 14600
+// bf16 tokens of 16 + 8 + 8 heads against 44, bound by the shuffles.) A warp takes L such pairs of vectors of one token at
+// a time. A block takes a run of such items; its tokens' sequences,
+// positions and pages (three loads that depend on one another) are looked up once, side by side, while the first items'
+// loads fly, and an item's loads are issued before the item ahead of it is worked on.
 #include "paged.cuh"
 
 namespace voxcuda {
@@ -26,7 +29,7 @@ struct AppendArgs {
     const float *qn, *kn, *cs;
     int64_t qkv_stride, q_stride;  // elements
     int64_t items;                 // tokens * groups of L warp loads
-    int32_t cs_rows, units;        // units: heads + 2 kv_heads
+    int32_t cs_rows, units, rounds; // units: heads + 2 kv_heads; rounds: items a warp
     FastDiv gdiv;                  // groups a token
     float eps;
 };
@@ -48,112 +51,151 @@ __device__ __forceinline__ void store_vals(T *p, const float (&v)[N]) {
     }
 }
 
+// Where a token's rows go: its position (-1: it is skipped) and page.
+struct TokenAt {
+    int pos, page;
+};
+__device__ __forceinline__ TokenAt token_at(const PagedArgs &p, int t) {
+    int b, pos;
+    bool ok = true;
+    if (p.q_start == nullptr) {
+        b = int(p.qdiv.div(uint32_t(t)));
+        pos = __ldg(p.kv_len + b) - p.q_per + t - b * p.q_per;
+    } else {
+        // the last sequence that starts at or before t; empty sequences share their start with the next
+        int lo = 0, hi = p.seqs;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (__ldg(p.q_start + mid) <= t) lo = mid + 1;
+            else hi = mid;
+        }
+        b = max(lo - 1, 0);
+        const int s0 = __ldg(p.q_start + b), s1 = __ldg(p.q_start + b + 1);
+        ok = t >= s0 && t < s1;
+        pos = int(int64_t(__ldg(p.kv_len + b)) - s1 + int64_t(t));
+    }
+    ok = ok && pos >= 0 && pos < p.cap;
+    int page = 0;
+    if (ok) {
+        page = __ldg(p.table + int64_t(b) * p.table_stride + (pos >> p.page_shift));
+        ok = uint32_t(page) < uint32_t(p.pages);
+    }
+    return {ok ? pos : -1, page};
+}
+
+constexpr int kRounds = 4;  // items a warp takes, at most
+
 template <typename QT, typename CT, int HD, int L>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendArgs a) {
     constexpr int V = 16 / int(sizeof(QT));  // elements a lane holds of a head
-    constexpr int LPH = HD / V;              // lanes a head
-    constexpr int HPW = 32 / LPH;            // heads a warp load
+    constexpr int LPH = HD / (2 * V);        // lanes a head
+    constexpr int HPW = 32 / LPH;            // heads a warp takes at once
+    __shared__ TokenAt at[kWarps * kRounds + 1];
     pdl_enter();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int e0 = (lane % LPH) * V, sub = lane / LPH;
-    const bool second = e0 >= HD / 2;  // this lane holds b; its partner holds a
-    const int p0 = second ? e0 - HD / 2 : e0;
-    const int64_t nw = int64_t(gridDim.x) * kWarps;
-    for (int64_t it = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5; it < a.items; it += nw) {
-        const uint32_t t = a.gdiv.div(uint32_t(it));
-        const int h0 = int(uint32_t(it) - t * a.gdiv.d) * (L * HPW) + sub;
+    const uint32_t i0 = blockIdx.x * uint32_t(kWarps * a.rounds), i1 = min(i0 + uint32_t(kWarps * a.rounds), uint32_t(a.items));
+    const uint32_t t0 = a.gdiv.div(i0);
+    uint4 raw[L][2];
+    auto fetch = [&](uint32_t it) {
+        const uint32_t t = a.gdiv.div(it);
+        const int h0 = int(it - t * a.gdiv.d) * (L * HPW) + sub;
         const QT *src = static_cast<const QT *>(a.qkv) + int64_t(t) * a.qkv_stride + int64_t(h0) * HD + e0;
-        uint4 raw[L];
 #pragma unroll
         for (int j = 0; j < L; ++j)
-            if (h0 + j * HPW < a.units) raw[j] = ld_stream(src + j * HPW * HD);
-        // the token's sequence and position
-        int b, pos;
-        bool ok = true;
-        if (a.p.q_start == nullptr) {
-            b = int(a.p.qdiv.div(t));
-            const int n = __ldg(a.p.kv_len + b);
-            pos = n - a.p.q_per + int(t - uint32_t(b) * uint32_t(a.p.q_per));
-        } else {
-            // the number of sequences that start at or before t, less one; empty sequences share their start with the next
-            int c = 0;
-            for (int i = lane; i < a.p.seqs; i += 32) c += __ldg(a.p.q_start + i) <= int(t);
-            b = __reduce_add_sync(0xffffffffu, c) - 1;
-            ok = b >= 0;
-            b = max(b, 0);
-            const int s0 = __ldg(a.p.q_start + b), s1 = __ldg(a.p.q_start + b + 1), n = __ldg(a.p.kv_len + b);
-            ok = ok && int(t) >= s0 && int(t) < s1;
-            pos = int(int64_t(n) - s1 + int64_t(t));
-        }
-        ok = ok && pos >= 0 && pos < a.p.cap && pos < a.cs_rows;
-        int page = 0;
-        if (ok) {
-            page = __ldg(a.p.table + int64_t(b) * a.p.table_stride + (pos >> a.p.page_shift));
-            ok = uint32_t(page) < uint32_t(a.p.pages);
-        }
-        if (!ok) {  // warp-uniform: the token is skipped
-            if (lane == 0) range_error();
-            continue;
-        }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) raw[j][y] = h0 + j * HPW < a.units ? ld_stream(src + j * HPW * HD + y * (HD / 2)) : make_uint4(0, 0, 0, 0);
+    };
+    uint32_t it = i0 + warp;
+    if (it < i1) fetch(it);
+    if (threadIdx.x <= a.gdiv.div(i1 - 1) - t0) {
+        TokenAt x = token_at(a.p, int(t0 + threadIdx.x));
+        if (x.pos >= a.cs_rows) x.pos = -1;
+        if (x.pos < 0) range_error();  // the token is skipped
+        at[threadIdx.x] = x;
+    }
+    __syncthreads();
+    for (; it < i1; it += kWarps) {
+        const uint32_t t = a.gdiv.div(it);
+        const int h0 = int(it - t * a.gdiv.d) * (L * HPW) + sub;
+        const TokenAt x_at = at[t - t0];
+        uint4 cur[L][2];
+#pragma unroll
+        for (int j = 0; j < L; ++j) cur[j][0] = raw[j][0], cur[j][1] = raw[j][1];
+        if (it + kWarps < i1) fetch(it + kWarps);
+        if (x_at.pos < 0) continue;
         float cs[2 * V];
-        const float4 *csr = reinterpret_cast<const float4 *>(a.cs + (int64_t(pos) * (HD / 2) + p0) * 2);
+        const float4 *csr = reinterpret_cast<const float4 *>(a.cs + (int64_t(x_at.pos) * (HD / 2) + e0) * 2);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
             const float4 c4 = __ldg(csr + i);
             cs[4 * i] = c4.x, cs[4 * i + 1] = c4.y, cs[4 * i + 2] = c4.z, cs[4 * i + 3] = c4.w;
         }
-        const int64_t row = int64_t(page) * a.p.page_stride + int64_t(pos & a.p.page_mask) * a.p.row_stride + e0;
+        const int64_t row = int64_t(x_at.page) * a.p.page_stride + int64_t(x_at.pos & a.p.page_mask) * a.p.row_stride + e0;
         QT *qrow = static_cast<QT *>(a.q) + int64_t(t) * a.q_stride + e0;
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             const int h = h0 + j * HPW;
-            float x[V];
-            Vec<DtOf<QT>::v>::unpack(h < a.units ? raw[j] : make_uint4(0, 0, 0, 0), x);
+            float x[2][V];
+            Vec<DtOf<QT>::v>::unpack(cur[j][0], x[0]);
+            Vec<DtOf<QT>::v>::unpack(cur[j][1], x[1]);
             const bool is_q = h < a.p.heads, is_v = h >= a.p.heads + a.p.kv_heads;
             const float *w = is_q ? a.qn : a.kn;
-            float ss = 0.f;
+            if (a.qn != nullptr || a.kn != nullptr) {
+                float s0 = 0.f, s1 = 0.f;  // the halves first, then across lanes: vox_cuda_qkv_rope's order at f32 heads of 128
 #pragma unroll
-            for (int e = 0; e < V; ++e) ss = fmaf(x[e], x[e], ss);
+                for (int e = 0; e < V; ++e) s0 = fmaf(x[0][e], x[0][e], s0), s1 = fmaf(x[1][e], x[1][e], s1);
+                float ss = s0 + s1;
 #pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (w != nullptr && !is_v) {  // hd is a power of two, so ss * (1 / hd) is ss / hd
-                const float inv = rsqrtf(fmaf(ss, 1.0f / float(HD), a.eps));
+                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (w != nullptr && !is_v) {  // hd is a power of two, so ss * (1 / hd) is ss / hd
+                    const float inv = rsqrtf(fmaf(ss, 1.0f / float(HD), a.eps));
 #pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                    const float4 w4 = __ldg(reinterpret_cast<const float4 *>(w + e0 + e));
-                    x[e] = __fmul_rn(w4.x, __fmul_rn(x[e], inv)), x[e + 1] = __fmul_rn(w4.y, __fmul_rn(x[e + 1], inv));
-                    x[e + 2] = __fmul_rn(w4.z, __fmul_rn(x[e + 2], inv)), x[e + 3] = __fmul_rn(w4.w, __fmul_rn(x[e + 3], inv));
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int e = 0; e < V; e += 4) {
+                            const float4 w4 = __ldg(reinterpret_cast<const float4 *>(w + e0 + y * (HD / 2) + e));
+                            x[y][e] = __fmul_rn(w4.x, __fmul_rn(x[y][e], inv)), x[y][e + 1] = __fmul_rn(w4.y, __fmul_rn(x[y][e + 1], inv));
+                            x[y][e + 2] = __fmul_rn(w4.z, __fmul_rn(x[y][e + 2], inv)), x[y][e + 3] = __fmul_rn(w4.w, __fmul_rn(x[y][e + 3], inv));
+                        }
                 }
             }
-            float o[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float other = __shfl_xor_sync(0xffffffffu, x[e], LPH / 2);
-                const float c = cs[2 * e], s = cs[2 * e + 1];
-                o[e] = second ? __fadd_rn(__fmul_rn(x[e], c), __fmul_rn(other, s)) : __fsub_rn(__fmul_rn(x[e], c), __fmul_rn(other, s));
-            }
             if (h >= a.units) continue;
-            if (is_q)
-                store_vals<QT, V>(qrow + int64_t(h) * HD, o);
-            else if (!is_v)
-                store_vals<CT, V>(static_cast<CT *>(a.p.k) + row + int64_t(h - a.p.heads) * a.p.head_stride, o);
-            else
-                store_vals<CT, V>(static_cast<CT *>(a.p.v) + row + int64_t(h - a.p.heads - a.p.kv_heads) * a.p.head_stride, x);
+            if (!is_v) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float c = cs[2 * e], s = cs[2 * e + 1], p = x[0][e], q = x[1][e];
+                    x[0][e] = __fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s));
+                    x[1][e] = __fadd_rn(__fmul_rn(q, c), __fmul_rn(p, s));
+                }
+            }
+            if (is_q) {
+                QT *dst = qrow + int64_t(h) * HD;
+                store_vals<QT, V>(dst, x[0]);
+                store_vals<QT, V>(dst + HD / 2, x[1]);
+            } else {
+                CT *dst = is_v ? static_cast<CT *>(a.p.v) + row + int64_t(h - a.p.heads - a.p.kv_heads) * a.p.head_stride
+                               : static_cast<CT *>(a.p.k) + row + int64_t(h - a.p.heads) * a.p.head_stride;
+                store_vals<CT, V>(dst, x[0]);
+                store_vals<CT, V>(dst + HD / 2, x[1]);
+            }
         }
     }
 }
 
 template <typename QT, typename CT, int HD>
 int launch_append(AppendArgs &a, cudaStream_t st) {
-    constexpr int HPW = 32 / (HD / (16 / int(sizeof(QT))));
-    const int loads = (a.units + HPW - 1) / HPW;  // warp loads a token
-    // Four loads in flight a warp where there are warps enough for the device either way, one where there are not
+    constexpr int HPW = 32 / (HD / (32 / int(sizeof(QT))));
+    const int loads = (a.units + HPW - 1) / HPW;  // warp steps a token
+    // Two pairs of loads an item and four items a warp where there are warps enough for the device either way, else one of each
     const bool many = int64_t(a.p.tokens) * loads >= int64_t(sm_count()) * 64;
-    const int L = many ? 4 : 1, groups = (loads + L - 1) / L;
+    const int L = many ? 2 : 1, groups = (loads + L - 1) / L;
+    a.rounds = many ? kRounds : 1;
     a.items = int64_t(a.p.tokens) * groups;
     a.gdiv = FastDiv(uint32_t(groups));
-    auto kern = many ? kv_append_kernel<QT, CT, HD, 4> : kv_append_kernel<QT, CT, HD, 1>;
-    launch_k(kern, balanced_grid(a.items, kWarps, resident_blocks((const void *)kern, kThreads, 0)), kThreads, 0, st, a);
+    auto kern = many ? kv_append_kernel<QT, CT, HD, 2> : kv_append_kernel<QT, CT, HD, 1>;
+    const int64_t per = int64_t(kWarps) * a.rounds;
+    launch_k(kern, dim3(unsigned((a.items + per - 1) / per)), kThreads, 0, st, a);
     return check_launch("vox_cuda_kv_append");
 }
 

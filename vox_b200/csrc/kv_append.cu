@@ -10,7 +10,7 @@
 // token) and by latency at single tokens. Layout: a lane holds a 16-byte vector of a head's first half and the one hd/2
 // further on, the rotation's partners, so the rotation stays in the lane and a head of width hd takes hd / 2V lanes (V = 4
 // f32 or 8 bf16); only the mean square crosses lanes. (One vector a lane, the partner fetched by shuffles: 61 us at 14600
-// bf16 tokens of 16 + 8 + 8 heads against 44, bound by the shuffles.) A warp takes L such pairs of vectors of one token at
+// bf16 tokens of 16 + 8 + 8 heads against 47, 5.3 TB/s, bound by the shuffles.) A warp takes L such pairs of vectors of one token at
 // a time. A block takes a run of such items; its tokens' sequences,
 // positions and pages (three loads that depend on one another) are looked up once, side by side, while the first items'
 // loads fly, and an item's loads are issued before the item ahead of it is worked on.
@@ -19,7 +19,7 @@
 namespace voxcuda {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 
 struct AppendArgs {
@@ -83,7 +83,7 @@ __device__ __forceinline__ TokenAt token_at(const PagedArgs &p, int t) {
     return {ok ? pos : -1, page};
 }
 
-constexpr int kRounds = 4;  // items a warp takes, at most
+constexpr int kRounds = 2;  // items a warp takes, at most
 
 template <typename QT, typename CT, int HD, int L>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendArgs a) {
@@ -187,13 +187,14 @@ template <typename QT, typename CT, int HD>
 int launch_append(AppendArgs &a, cudaStream_t st) {
     constexpr int HPW = 32 / (HD / (32 / int(sizeof(QT))));
     const int loads = (a.units + HPW - 1) / HPW;  // warp steps a token
-    // Two pairs of loads an item and four items a warp where there are warps enough for the device either way, else one of each
+    // Four pairs of loads an item and two items a warp (47 us at the size above; two pairs and four items 50) where there are
+    // warps enough for the device either way, else one of each
     const bool many = int64_t(a.p.tokens) * loads >= int64_t(sm_count()) * 64;
-    const int L = many ? 2 : 1, groups = (loads + L - 1) / L;
+    const int L = many ? 4 : 1, groups = (loads + L - 1) / L;
     a.rounds = many ? kRounds : 1;
     a.items = int64_t(a.p.tokens) * groups;
     a.gdiv = FastDiv(uint32_t(groups));
-    auto kern = many ? kv_append_kernel<QT, CT, HD, 2> : kv_append_kernel<QT, CT, HD, 1>;
+    auto kern = many ? kv_append_kernel<QT, CT, HD, 4> : kv_append_kernel<QT, CT, HD, 1>;
     const int64_t per = int64_t(kWarps) * a.rounds;
     launch_k(kern, dim3(unsigned((a.items + per - 1) / per)), kThreads, 0, st, a);
     return check_launch("vox_cuda_kv_append");

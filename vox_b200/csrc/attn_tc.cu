@@ -1,17 +1,17 @@
 // The paged attention of many query rows on the 5th-generation tensor cores (bf16 activations on a bf16 cache).
 //
 // A block takes up to two tiles of 128 query rows of one key/value head (row = token * group + query head in the group, so
-// the heads that share keys share every tile of K and V) and walks the keys in tiles of 128: S = Q K^T (M 128, N 128 keys)
-// and O += P V (M 128, N hd), both accumulated in f32 in tensor memory; P (bf16) overwrites the upper half of its S
-// columns, from where the second product reads it as its A operand. TMEM: S0 S1 at columns 0 and 128, O0 O1 at 256.
+// the heads that share keys share every tile of K and V) and walks the keys: S = Q K^T (M 128, N 64 keys) and O += P V (M 128,
+// N hd, K 64 keys), both accumulated in f32 in tensor memory; P (bf16) overwrites the first half of its S columns, from where
+// the second product reads it as its A operand. Every row tile has two S buffers, so the next scores are there when a
+// softmax step ends: the products are off its path. TMEM: S of row tile q, buffer b at column 128 q + 64 b; O at 256 + hd q.
 //   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row. Online softmax with a lazy reference: the row's reference
 //                   maximum moves only when a score exceeds it by 8 (in powers of two: weights stay below 256, far from
-//                   any overflow), so O is rescaled in the few tiles where it does; exact, since numerator and
+//                   any overflow), so O is rescaled in the few steps where it does; exact, since numerator and
 //                   denominator always share the reference.
-//   warp 8          tensor copies of K and V tiles through a ring of stages, page by page (a box never leaves a page);
-//                   rows of V past the last key are zeroed (their weight is 0, and 0 times what lies there may be NaN)
-//   warp 9          issues the MMAs (warps 10 and 11 only complete the warpgroup that gives its registers away): P V of a tile, then Q K^T of the next tile of the same rows, alternating between the
-//                   two row tiles, so that one tile's softmax runs while the other's products do.
+//   warp 8          tensor copies of K and V tiles of 128 keys through a ring of stages, page by page (a box never leaves a
+//                   page); rows of V past the last key are zeroed (their weight is 0, and 0 times what lies there may be NaN)
+//   warps 9, 10     issue the products of row tile 0, 1: P V of a step, then Q K^T two steps on into the same S buffer
 // Tile order in the ring: K0 V0 K1 V1 ... (both row tiles read each). Every wait is bounded.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -25,12 +25,12 @@
 namespace voxcuda {
 namespace {
 
-constexpr int kKeys = 128;
-constexpr int kTcThreads = 384;
-constexpr int kTcRegs = 168;  // registers a thread at launch; 2 x 200 + 104 = 3 x 168 after the split below
+constexpr int kKeys = 128;  // keys a stage; a softmax step takes half of them
+constexpr int kStepKeys = 64;
+constexpr int kTcThreads = 352;
 constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 
-constexpr int POLY = 0x10;  // which of eight pairs of weights take ex2_poly
+constexpr int POLY = 0x11;  // which of eight pairs of weights take ex2_poly
 
 constexpr int tc_stages(int hd) { return hd == 128 ? 5 : 8; }
 constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }
@@ -53,18 +53,13 @@ __device__ __forceinline__ void umma_qk_warp(uint32_t d, uint64_t da, uint64_t d
                      "l"(db), "r"(idesc), "r"(smem_addr(bar))
                      : "memory");
 }
-// O (+)= P V, 16 keys a step: P in TMEM (two bf16 a column: 8 columns a step), V MN-major (2048 bytes a step). The first six
-// steps (acc: whether O holds something), and the last two.
+// O (+)= P V over 64 keys, 16 a step: P in TMEM (two bf16 a column: 8 columns a step), V MN-major (2048 bytes a step); acc:
+// whether O holds something.
 #define VOX_PV_STEP(C, OFF, P) "add.s32 a, %1, " C ";\n\tadd.s64 b, %2, " OFF ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, " P ";\n\t"
-__device__ __forceinline__ void umma_pv_first_warp(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred e, p, o;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 o, 0, 0;\n\t"
+__device__ __forceinline__ void umma_pv_warp(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc, uint64_t *bar) {
+    asm volatile("{\n\t.reg .pred e, p, o;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 o, 0, 0;\n\t"
                  VOX_PV_STEP("0", "0", "p") VOX_PV_STEP("8", "128", "o") VOX_PV_STEP("16", "256", "o") VOX_PV_STEP("24", "384", "o")
-                 VOX_PV_STEP("32", "512", "o") VOX_PV_STEP("40", "640", "o") "}" ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(acc)
-                 : "memory");
-}
-__device__ __forceinline__ void umma_pv_rest_warp(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc) {
-    asm volatile("{\n\t.reg .pred e, o;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.eq.b32 o, 0, 0;\n\t"
-                 VOX_PV_STEP("48", "768", "o") VOX_PV_STEP("56", "896", "o") "}" ::"r"(d), "r"(ta), "l"(db), "r"(idesc)
+                 VOX_COMMIT ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(smem_addr(bar)), "r"(acc)
                  : "memory");
 }
 // 16 consecutive columns of this thread's TMEM lane.
@@ -170,22 +165,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     constexpr int NS = tc_stages(HD), H = HD / 64;
     constexpr uint32_t kTile = H * kHalf;
-    constexpr uint32_t kIdS = umma_idesc_bf16(128, kKeys), kIdO = umma_idesc_bf16(128, HD, true);
+    constexpr uint32_t kIdS = umma_idesc_bf16(128, kStepKeys), kIdO = umma_idesc_bf16(128, HD, true);
     extern __shared__ uint8_t raw[];
     __shared__ TcJob job;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sQ = smem_addr(smem), sKV = sQ + 2 * kTile;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + (2 + NS) * kTile), *empty = full + NS;
-    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *p_rest = p_full + 2, *o_full = p_rest + 2, *q_full = o_full + 2, *tail = q_full + 2, *drain = tail + 1;
+    uint64_t *s_full = empty + NS, *p_full = s_full + 4, *o_done = p_full + 4, *o_full = o_done + 2, *q_full = o_full + 2, *tail = q_full + 2, *drain = tail + 1;
     uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_enter();
     if (warp == 0) tc_job(a, blockIdx.x, job);
     if (threadIdx.x == 32) {
-        for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int q = 0; q < 2; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 4), mbar_init(&p_rest[q], 4), mbar_init(&q_full[q], 4), mbar_init(&o_full[q], 1);
+        for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 2);
+        for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+        for (int q = 0; q < 2; ++q) mbar_init(&q_full[q], 4), mbar_init(&o_done[q], 1), mbar_init(&o_full[q], 1);
         mbar_init(tail, 1);
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);
         mbar_init_fence();
     }
     if (warp == 9) tmem_alloc(tslot, 512);
@@ -198,7 +194,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (warp == 9) tmem_dealloc(tmem, 512);
         return;
     }
-    // key tiles: nA of the prefix, then the own keys from kb0; hi of a row tile = keys that its last row sees
+    // key tiles of 128: nA of the prefix, then the own keys from kb0; hi of a row tile = keys that its last row sees; nt = its
+    // steps of 64 keys
     const int nA = (j.pa1 - j.pa0 + kKeys - 1) / kKeys;
     int kb0 = j.k0;
     if (a.window > 0 && j.causal) {
@@ -213,14 +210,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (r0 < j.rows && 128 * q < a.tc_rows) {
             const int last = int(a.gdiv.div(uint32_t(min(r0 + 127, j.rows - 1))));
             const int hi = j.causal ? min(j.base + last + 1, j.k1) : 0;
-            nt[q] = nA + max(hi - kb0 + kKeys - 1, 0) / kKeys;
+            nt[q] = 2 * nA + max(hi - kb0 + kStepKeys - 1, 0) / kStepKeys;
             kend = max(kend, hi);
         }
     }
-    const int nmax = max(nt[0], nt[1]);
+    const int nmax = (max(nt[0], nt[1]) + 1) / 2;  // tiles of 128
     if (warp < 8) {
         // ---------------------------------------------------------------- softmax: thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         {   // the row tile's Q: 16-byte chunks of whole rows, every load in flight before the first is stored, 128-byte
             // swizzle; rows past the end are zero
             const int q = warp >> 2, w = warp & 3;
@@ -250,8 +246,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         const int q = warp >> 2, row = (warp & 3) * 32 + lane, rr = j.row0 + 128 * q + row;
         const int n = q ? nt[1] : nt[0];
-        const uint32_t tS = tmem + (uint32_t((warp & 3) * 32) << 16) + 128 * q, tP = tS + 64;
-        const uint32_t tO = tmem + (uint32_t((warp & 3) * 32) << 16) + 256 + HD * q;
+        const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16), tO = lanes + 256 + HD * q;
         const bool live = rr < j.rows && 128 * q < a.tc_rows;
         const int i_tok = int(a.gdiv.div(uint32_t(live ? rr : 0)));
         const int hi_own = live && j.causal ? min(j.base + i_tok + 1, j.k1) : 0;
@@ -259,33 +254,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float ref = -INFINITY;  // reference maximum (scaled, base 2)
         float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         bool ok = true;
-        for (int i = 0; i < n && ok; ++i) {
-            ok = wait_soon(&s_full[q], uint32_t(i & 1));
+#pragma unroll 1
+        for (int u = 0; u < n; ++u) {
+            const uint32_t tS = lanes + 128 * q + 64 * (u & 1);
+            ok = wait_soon(&s_full[2 * q + (u & 1)], uint32_t(u >> 1) & 1u);
             if (!ok) break;
             tc_fence_after();
-            uint32_t r[128];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
-            const bool pre = i < nA;
-            const int key0 = pre ? j.pa0 + i * kKeys : kb0 + (i - nA) * kKeys;
+            uint32_t r[64];
+            tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(r));
+            tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+            tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r));
+            tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
+            const bool pre = u < 2 * nA;
+            const int key0 = pre ? j.pa0 + u * kStepKeys : kb0 + (u - 2 * nA) * kStepKeys;
             const int hi = (pre ? (live ? j.pa1 : 0) : hi_own) - key0, lo = (pre ? j.pa0 : lo_own) - key0;
-            if (!__all_sync(0xffffffffu, hi >= kKeys && lo <= 0)) {
+            if (!__all_sync(0xffffffffu, hi >= kStepKeys && lo <= 0)) {
 #pragma unroll
-                for (int c = 0; c < kKeys; ++c)
+                for (int c = 0; c < kStepKeys; ++c)
                     if (c >= hi || c < lo) r[c] = __float_as_uint(-INFINITY);
             }
-            float m8[8];
+            float m4[4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) m8[c] = max3(__uint_as_float(r[c]), __uint_as_float(r[c + 8]), __uint_as_float(r[c + 16]));
+            for (int c = 0; c < 4; ++c) m4[c] = max3(__uint_as_float(r[c]), __uint_as_float(r[c + 4]), __uint_as_float(r[c + 8]));
 #pragma unroll
-            for (int c = 24; c < kKeys - 8; c += 16)
+            for (int c = 12; c < 60; c += 8)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m8[e] = max3(m8[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 8 + e]));
+                for (int e = 0; e < 4; ++e) m4[e] = max3(m4[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m8[e] = fmaxf(m8[e], __uint_as_float(r[kKeys - 8 + e]));
-            const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * a.tc_scale;
+            for (int e = 0; e < 4; ++e) m4[e] = fmaxf(m4[e], __uint_as_float(r[60 + e]));
+            const float mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * a.tc_scale;
             const bool move = mx > ref + 8.0f;  // also the first key that the row sees (ref = -inf)
             if (__any_sync(0xffffffffu, move)) {
                 const float nref = move ? mx : ref;
@@ -293,47 +290,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ref = nref;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) l2[e] = mul2(l2[e], bc2(alpha));
-                if (i > 0) {  // the arrival of this S implies that the P V before it has completed
+                if (u > 0) {  // the step before's P V has to be in O first (these scores came behind the one before that)
+                    ok = wait_soon(&o_done[q], uint32_t(u - 1) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + c, o);
+                        tmem_wait_ld(o);
 #pragma unroll
-                    for (int c = 0; c < HD / 16; ++c) {
-                        uint32_t o[16];
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                                     : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
-                                       "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                                     : "r"(tO + 16 * c)
-                                     : "memory");
-                        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                                     : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]), "+r"(o[8]),
-                                       "+r"(o[9]), "+r"(o[10]), "+r"(o[11]), "+r"(o[12]), "+r"(o[13]), "+r"(o[14]), "+r"(o[15])
-                                     :
-                                     : "memory");
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st16(tO + 16 * c, o);
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st16(tO + c, *reinterpret_cast<uint32_t(*)[16]>(o));
+                        tmem_st16(tO + c + 16, *reinterpret_cast<uint32_t(*)[16]>(o + 16));
                     }
                 }
             }
             const float2 sc = bc2(a.tc_scale), nr = bc2(ref == -INFINITY ? 0.f : -ref);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int k = 32 * c + 2 * e;
                     const float2 x = fma2(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), sc, nr);
-                    // part of the weights on the multiply-add pipe: the special-function unit alone would take all of a tile
+                    // part of the weights on the multiply-add pipe: the special-function unit alone would take all of a step
                     const float2 p = (POLY >> (e & 7)) & 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
                     l2[e & 3] = add2(l2[e & 3], p);
                     w[e] = pack_bf16(p.x, p.y);
                 }
-                tmem_st16(tP + 16 * c, w);
-                if (c >= 2) {  // three quarters of the weights, then the rest: the second product starts on what is there
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(c == 2 ? &p_full[q] : &p_rest[q]);
-                }
+                tmem_st16(tS + 16 * c, w);
             }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * q + (u & 1)]);
         }
         if (n > 0 && ok) {
             ok = wait_soon(&o_full[q], 0);
@@ -400,9 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
         }
         if (live && ok && a.partial) a.part_ml[slot] = make_float2(ref, l);
-    } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == 8) {
+    } else if (warp == 8) {
         // ---------------------------------------------------------------- copies
         const int pr = min(a.p.page_mask + 1, kKeys);  // rows a box
         bool ok = true;
@@ -438,59 +427,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         // every copy issued has landed before the block's shared memory is released
         for (int m = max(n - NS, 0); m < n; ++m) wait_soon(&full[m % NS], uint32_t(m / NS) & 1u);
-    } else if (warp == 9) {
-        // ---------------------------------------------------------------- MMAs
+    } else {
+        // ---------------------------------------------------------------- products of row tile q
+        const int q = warp - 9, n = q ? nt[1] : nt[0];
         bool ok = true;
         auto wait_full = [&](int m) { return wait_soon(&full[m % NS], uint32_t(m / NS) & 1u); };
-        const uint64_t dQ = umma_desc(sQ, 16, 1024), dK = umma_desc(sKV, 16, 1024), dV = umma_desc(sKV, kHalf, 1024);
-        constexpr uint32_t kStep = kTile >> 4;  // a tile on, in descriptor units
-        auto qk = [&](int q, int st) { umma_qk_warp<HD>(tmem + 128 * q, dQ + uint32_t(q) * kStep, dK + uint32_t(st) * kStep, kIdS, &s_full[q]); };
-        if (nmax > 0) {
-            ok = wait_full(0);
+        constexpr uint32_t kStep = kTile >> 4, kSub = kStepKeys * 128 >> 4;  // a tile, half a tile's rows on, in descriptor units
+        const uint64_t dQ = umma_desc(sQ + q * kTile, 16, 1024), dK = umma_desc(sKV, 16, 1024), dV = umma_desc(sKV, kHalf, 1024);
+        const uint32_t tS = tmem + 128 * q, tO = tmem + 256 + HD * q;
+        auto qk = [&](int u) {  // scores of step u; the last step of a tile gives K back
+            const int m = u & ~1;
+            if (!(u & 1)) ok = wait_full(m);
+            if (!ok) return;
             tc_fence_after();
-            if (ok) {
-#pragma unroll 1
-                for (int q = 0; q < 2 && ok; ++q)
-                    if ((q ? nt[1] : nt[0]) > 0) {
-                        ok = wait_soon(&q_full[q], 0);
-                        tc_fence_after();
-                        if (ok) qk(q, 0);
-                    }
-                umma_commit_warp(&empty[0]);
-            }
+            umma_qk_warp<HD>(tS + 64 * (u & 1), dQ, dK + uint32_t(m % NS) * kStep + (u & 1) * kSub, kIdS, &s_full[2 * q + (u & 1)]);
+            if ((u & 1) || u + 1 == n) umma_commit_warp(&empty[m % NS]);
+        };
+        if (n > 0) {
+            ok = wait_soon(&q_full[q], 0);
+            if (ok) qk(0);
+            if (ok && n > 1) qk(1);
         }
 #pragma unroll 1
-        for (int i = 0; i < nmax && ok; ++i) {
-            const int nv = 2 * i + 1, sv = nv % NS, sk = (nv + 1) % NS;
-            ok = wait_full(nv);  // V of this tile, usually there long before P
-            if (i + 1 < nmax) ok = ok && wait_full(nv + 1);
-#pragma unroll 1
-            for (int q = 0; q < 2 && ok; ++q) {
-                const int n = q ? nt[1] : nt[0];
-                if (i >= n) continue;
-                const uint32_t tO = tmem + 256 + HD * q, tP = tmem + 128 * q + 64;
-                ok = wait_soon(&p_full[q], uint32_t(i & 1));
-                if (!ok) break;
-                tc_fence_after();
-                umma_pv_first_warp(tO, tP, dV + uint32_t(sv) * kStep, kIdO, uint32_t(i > 0));
-                ok = wait_soon(&p_rest[q], uint32_t(i & 1));
-                if (!ok) break;
-                tc_fence_after();
-                umma_pv_rest_warp(tO, tP, dV + uint32_t(sv) * kStep, kIdO);
-                if (i + 1 < n)
-                    qk(q, sk);
-                else
-                    umma_commit_warp(&o_full[q]);
-            }
-            if (ok) {
-                umma_commit_warp(&empty[sv]);
-                if (i + 1 < nmax) umma_commit_warp(&empty[sk]);
-            }
+        for (int u = 0; u < n && ok; ++u) {
+            const int m = u | 1;  // V of the tile
+            if (!(u & 1)) ok = wait_full(m);
+            ok = ok && wait_soon(&p_full[2 * q + (u & 1)], uint32_t(u >> 1) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            umma_pv_warp(tO, tS + 64 * (u & 1), dV + uint32_t(m % NS) * kStep + (u & 1) * kSub, kIdO, uint32_t(u > 0), &o_done[q]);
+            if ((u & 1) || u + 1 == n) umma_commit_warp(&empty[m % NS]);
+            if (u + 1 == n) umma_commit_warp(&o_full[q]);
+            if (u + 2 < n) qk(u + 2);
         }
-        umma_commit_warp(drain);  // every MMA issued has completed before the tensor memory is released
+        // tiles that only the other row tile reads: given back as they come (a stage is free when both warps have said so)
+        for (int m = (n + 1) / 2 * 2; m < 2 * nmax && ok; ++m) {
+            ok = wait_full(m);
+            if (ok && lane == 0) mbar_arrive(&empty[m % NS]);
+        }
+        umma_commit_warp(drain);  // every product issued has completed before the tensor memory is released
         __syncwarp();
         wait_soon(drain, 0);
-    }
     }
     tc_fence_before();
     __syncthreads();
@@ -517,12 +494,6 @@ PFN_cuTensorMapEncodeTiled_v12000 encode() {
 template <int HD>
 int launch(const AttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int64_t blocks, cudaStream_t st, const char *name) {
     auto kern = attn_tc_kernel<HD>;
-    // the kernel hands registers between its warpgroups: their sum must be what it was launched with
-    static const int regs = [] {
-        cudaFuncAttributes at = {};
-        return cudaFuncGetAttributes(&at, (const void *)attn_tc_kernel<HD>) == cudaSuccess ? at.numRegs : -1;
-    }();
-    if (regs != kTcRegs) return set_error(VOX_CUDA_ERR_DEVICE, std::string(name) + ": unexpected register count of the tensor-core kernel");
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tc_smem(HD))) != cudaSuccess) return check_launch(name);
     launch_k(kern, dim3(unsigned(blocks)), kTcThreads, tc_smem(HD), st, a, mk, mv);
     return check_launch(name);

@@ -464,3 +464,121 @@ def test_refusals(vox):
     # no page listed: no key, zeros
     out = kv.attend(torch.ones((1, 128), device="cuda"), z(1, 0, dt=torch.int32), n1)
     assert bool((out == 0).all())
+
+
+# ------------------------------------------------------------------ the ways a call is cut
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 128), (7, 1, 64)])
+@pytest.mark.parametrize("prefix", [0, 140])
+def test_many_sequences_share_the_blocks(vox, act, cache, heads, kvh, hd, prefix):
+    """More sequences than a block has threads, lengths from 0 to several tiles: equal runs of all sequences' tiles, with and
+    without offsets of the tokens, sequences without new tokens and without keys among them."""
+    rng = np.random.default_rng(5)
+    kv = [int(x) for x in rng.integers(0, 260, 300)]
+    kv[0], kv[7], kv[8], kv[299] = 1500, 0, 0, 1
+    bt = Batch([(1, n) for n in kv], kvh, hd, 16, cache, seed=1, prefix=prefix)
+    q = queries(bt, heads, act)
+    table, kv_len, _ = bt.dev(uniform=True)
+    h = bt.handle(vox)
+    call = (lambda **k: h.attend_prefix(q.cuda(), bt.prefix_pages.cuda(), prefix, table, kv_len, max_kv=1500, **k)) if prefix else \
+        (lambda **k: h.attend(q.cuda(), table, kv_len, max_kv=1500, **k))
+    want, mag, big = attention64(bt, q, heads, hd ** -0.5)
+    check(call(), want, mag, big, act, cache, 1700)
+    got = call(q_start=bt.q_start.cuda(), max_q=1)
+    check(got, want, mag, big, act, cache, 1700)
+    # some sequences have no new token, one has more than the host says (of rows for two blocks of the few-row kernels)
+    lens = [(int(x), n) for x, n in zip(rng.integers(0, 2, 300), kv)]
+    lens[0], lens[7], lens[40] = (21, 1500), (3, 0), (5, 3)
+    bt = Batch(lens, kvh, hd, 16, cache, seed=2, prefix=prefix)
+    q = queries(bt, heads, act)
+    table, kv_len, q_start = bt.dev()
+    h = bt.handle(vox)
+    got = call(q_start=q_start, max_q=1)
+    want, mag, big = attention64(bt, q, heads, hd ** -0.5)
+    check(got, want, mag, big, act, cache, 1700)
+    assert vox.device_error() == 0
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("window", [1, 50, 300])
+def test_window_over_many_sequences(vox, act, cache, window):
+    lens = [(1, int(n)) for n in np.random.default_rng(6).integers(1, 900, 90)]
+    bt = Batch(lens, 4, 128, 16, cache, seed=window)
+    q = queries(bt, 8, act)
+    table, kv_len, _ = bt.dev(uniform=True)
+    got = bt.handle(vox).attend(q.cuda(), table, kv_len, max_kv=3000, window=window)
+    want, mag, big = attention64(bt, q, 8, 128 ** -0.5, window)
+    check(got, want, mag, big, act, cache, 900)
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("page", [16, 64, 128, 512])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompts_of_several_row_blocks(vox, act, cache, page, hd):
+    """Prompts that continue cached rows, of several blocks of rows and tiles of keys, that end one row before, at and past
+    the ends of tiles, steps and pages."""
+    lens = [(257, 640), (128, 128), (129, 513), (64, 65), (1, 511), (300, 301)]
+    bt = Batch(lens, 2, hd, page, cache, seed=page)
+    q = queries(bt, 4, act)
+    table, kv_len, q_start = bt.dev()
+    h = bt.handle(vox)
+    want, mag, big = attention64(bt, q, 4, hd ** -0.5)
+    for mq, mkv in ((300, 640), (0, 0)):
+        check(h.attend(q.cuda(), table, kv_len, q_start=q_start, max_q=mq, max_kv=mkv), want, mag, big, act, cache, 640)
+    want, mag, big = attention64(bt, q, 4, hd ** -0.5, window=100)
+    check(h.attend(q.cuda(), table, kv_len, q_start=q_start, max_q=300, window=100), want, mag, big, act, cache, 640)
+    assert vox.device_error() == 0
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("q", [1, 9, 70])
+def test_prefix_of_many_tiles(vox, act, cache, q):
+    """A prefix cut into several key ranges, against single tokens, short continuations and prompts."""
+    bt = Batch([(q, q), (q, q + 150)] * 9, 2, 128, 64, cache, seed=q, prefix=1000)
+    x = queries(bt, 4, act)
+    table, kv_len, q_start = bt.dev(uniform=True)
+    got = bt.handle(vox).attend_prefix(x.cuda(), bt.prefix_pages.cuda(), 1000, table, kv_len, max_kv=q + 150)
+    want, mag, big = attention64(bt, x, 4, 128 ** -0.5)
+    check(got, want, mag, big, act, cache, 1200)
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+def test_scores_that_keep_rising(vox, act, cache):
+    """Every step's largest score is far above the last one's, so the running maximum moves at each; and far below, so it
+    never does."""
+    for sign in (1.0, -1.0):
+        bt = Batch([(1, 700), (150, 700)], 2, 64, 16, cache, seed=7)
+        ramp = (torch.arange(700) / 700.0 * 40.0 * sign)[:, None, None]
+        for b in range(2):
+            p, r = bt.rows(bt.table[b], 700)
+            bt.k[p, r] = (torch.ones(700, 2, 64) * ramp / 8).to(cache)
+        q = torch.ones((bt.tokens, 4, 64)).to(act)
+        table, kv_len, q_start = bt.dev()
+        got = bt.handle(vox).attend(q.cuda(), table, kv_len, q_start=q_start, max_q=150)
+        want, mag, big = attention64(bt, q, 4, 64 ** -0.5)
+        check(got, want, mag, big, act, cache, 700)
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 80])
+def test_nan_in_a_query_or_key_reaches_its_rows_only(vox, act, cache, n):
+    """A query that holds NaN gives NaN in its own row; a key that holds NaN, in the rows that see it."""
+    bt = Batch([(n, 200), (n, 150)], 2, 64, 16, cache, seed=3)
+    q = queries(bt, 4, act)
+    table, kv_len, q_start = bt.dev()
+    clean = bt.handle(vox).attend(q.cuda(), table, kv_len, q_start=q_start, max_q=n)
+    bad = q.clone()
+    bad[n - 1, 2, 5] = math.nan
+    got = bt.handle(vox).attend(bad.cuda(), table, kv_len, q_start=q_start, max_q=n)
+    assert bool(torch.isnan(got[n - 1, 2]).all())
+    keep = torch.ones((2 * n, 4), dtype=torch.bool)
+    keep[n - 1, 2] = False
+    assert torch.equal(got[keep.cuda()], clean[keep.cuda()])
+    p, r = bt.rows(bt.table[1], 150)
+    bt.k[p[149], r[149], 0, 3] = math.nan  # the last key of the second sequence, key/value head 0: its last token alone sees it
+    got = bt.handle(vox).attend(q.cuda(), table, kv_len, q_start=q_start, max_q=n)
+    assert bool(torch.isnan(got[2 * n - 1, :2]).all())
+    keep = torch.ones((2 * n, 4), dtype=torch.bool)
+    keep[2 * n - 1, :2] = False
+    assert torch.equal(got[keep.cuda()], clean[keep.cuda()])

@@ -296,7 +296,7 @@ VOX_CUDA_API int vox_cuda_add_rmsnorm(void *h, const void *delta, const float *l
  * Pages and rows may lie in any order of memory that these strides give ([pages][page_size][kv_heads][head_dim], or
  * head-major, or one tensor that holds both); a linear cache is one page a sequence.
  *   dtype: VOX_CUDA_F32 or VOX_CUDA_BF16; page_size: a power of two, 16 .. 2^20; head_dim: 64 or 128 (the widths of the
- *   reference's talkers); strides in elements, each a multiple of 16 bytes; k and v 16-byte aligned.
+ *   reference's talkers); strides in elements, positive, each a multiple of 16 bytes; k and v 16-byte aligned.
  * No counterpart in the reference, whose caches are linear or rings of one sequence (appends in transformer_forward,
  * kernels.cpp:797-806; shaders/ringput.comp). */
 typedef struct vox_cuda_kv_cache {
@@ -342,8 +342,9 @@ VOX_CUDA_API int vox_cuda_kv_append(const vox_cuda_kv_cache *cache, const vox_cu
  * head h / (heads / kv_heads). Prompts and single tokens alike (q_len 0, 1 or more a sequence, mixed in a call).
  *   q, out [tokens][heads][hd], row strides q_stride / out_stride elements, `dtype` f32 or bf16; out must not overlap q
  * A token that sees no key gives zeros. Cache rows at or past kv_len are never used, whatever they hold; the rows below it
- * must be finite. f32 activations keep f32 accuracy (CUDA cores). bf16 activations on a bf16 cache run on the tensor cores
- * with f32 scores, statistics and sums; the weights are rounded to bf16 for the product with v (about 2^-9 relative).
+ * must be finite. Scores, softmax statistics and sums are f32. bf16 activations on a bf16 cache: the weights are rounded to
+ * bf16 for the product with v (2^-8 relative). Every other pair of types keeps f32 accuracy (about 1e-6): few rows on an f32
+ * cache run on the CUDA cores, the rest on the tensor cores with operands cut into parts whose products are exact to 2^-21.
  * Results are identical run to run. workspace: vox_cuda_attn_workspace bytes of scratch, 256-byte aligned (NULL where that
  * says 0), not shared by calls that can overlap. Replaces attention.comp:1-45 and the attention of transformer_forward
  * (kernels.cpp:809-828); window: attnw.comp:1-48. */

@@ -86,6 +86,22 @@ bool gpu_add_rmsnorm(void *h, const void *delta, const float *layer_scale, const
 bool gpu_matvec(bool q4, const void *codes, const void *scale, int scale_dtype, const float *bias, const float *x, float *y,
                 int64_t rows, int64_t cols, int64_t m, bool accumulate = false, void *stream = nullptr);
 
+// ---- paged key/value cache of a batch of sequences (the same steps for many streams at once) ----
+// Split, head RMSNorm, RoPE and cache write of the batch's new tokens (see vox_cuda_kv_append); qkv and q densely packed rows.
+bool gpu_kv_append(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const void *qkv, const float *qn, const float *kn,
+                   const float *cs, int64_t cs_rows, void *q, int64_t heads, float eps, int dtype = VOX_CUDA_F32, void *stream = nullptr);
+// Causal attention of the new tokens over their sequences' rows (kernels.cpp:809-828, attention.comp); q and out densely packed
+// rows; workspace of gpu_attn_workspace bytes.
+bool gpu_attn_paged(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const void *q, void *out, int64_t heads, float scale,
+                    int64_t window, void *workspace, size_t workspace_bytes, int dtype = VOX_CUDA_F32, void *stream = nullptr);
+// The same behind one prefix that all sequences share (a voice prompt), read once for the batch.
+bool gpu_attn_prefix(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const int32_t *prefix_pages, int64_t prefix_len,
+                     const void *q, void *out, int64_t heads, float scale, void *workspace, size_t workspace_bytes,
+                     int dtype = VOX_CUDA_F32, void *stream = nullptr);
+// Bytes of workspace of the two calls above (prefix_len 0: gpu_attn_paged); false: *bytes is not set.
+bool gpu_attn_workspace(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, int64_t prefix_len, int64_t heads, int64_t window,
+                        int dtype, size_t *bytes);
+
 // ---- host-pointer conveniences (copy in, run, copy out; synchronous) ----
 bool rmsnorm_host(const float *x, const float *w, int64_t rows, int64_t n, float eps, float *out);
 bool softmax_causal_host(const float *scores, float *probs, int64_t heads, int64_t q_len, int64_t n_keys, float scale);

@@ -166,6 +166,28 @@ VOX_CXX_API bool gpu_matvec(bool q4, const void *codes, const void *scale, int s
     return done(vox_cuda_gemv_q8(static_cast<const int8_t *>(codes), scale, scale_dtype, bias, x, y, rows, cols, m,
                                  accumulate ? 1 : 0, stream));
 }
+VOX_CXX_API bool gpu_kv_append(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const void *qkv, const float *qn,
+                               const float *kn, const float *cs, int64_t cs_rows, void *q, int64_t heads, float eps, int dtype,
+                               void *stream) {
+    return done(vox_cuda_kv_append(&cache, &batch, qkv, (heads + 2 * int64_t(cache.kv_heads)) * cache.head_dim, qn, kn, cs, cs_rows, q,
+                                   heads * cache.head_dim, heads, eps, dtype, stream));
+}
+VOX_CXX_API bool gpu_attn_paged(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const void *q, void *out, int64_t heads,
+                                float scale, int64_t window, void *workspace, size_t workspace_bytes, int dtype, void *stream) {
+    const int64_t row = heads * cache.head_dim;
+    return done(vox_cuda_attn_paged(&cache, &batch, q, row, out, row, heads, scale, window, dtype, workspace, workspace_bytes, stream));
+}
+VOX_CXX_API bool gpu_attn_prefix(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const int32_t *prefix_pages,
+                                 int64_t prefix_len, const void *q, void *out, int64_t heads, float scale, void *workspace,
+                                 size_t workspace_bytes, int dtype, void *stream) {
+    const int64_t row = heads * cache.head_dim;
+    return done(vox_cuda_attn_prefix(&cache, &batch, prefix_pages, prefix_len, q, row, out, row, heads, scale, dtype, workspace,
+                                     workspace_bytes, stream));
+}
+VOX_CXX_API bool gpu_attn_workspace(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, int64_t prefix_len, int64_t heads,
+                                    int64_t window, int dtype, size_t *bytes) {
+    return done(vox_cuda_attn_workspace(&cache, &batch, prefix_len, heads, window, dtype, bytes));
+}
 
 // ---- host-pointer conveniences ----
 

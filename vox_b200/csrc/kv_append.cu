@@ -211,7 +211,7 @@ int paged_args(const vox_cuda_kv_cache *c, const vox_cuda_kv_batch *b, int64_t h
                 std::string(name) + ": bad cache shape (heads must be a multiple of kv_heads)");
     if (c->head_dim != 64 && c->head_dim != 128) return set_error(VOX_CUDA_ERR_UNSUPPORTED, std::string(name) + ": head_dim must be 64 or 128");
     const int64_t el = 16 / dtype_size(c->dtype);
-    VOX_REQUIRE(c->page_stride % el == 0 && c->row_stride % el == 0 && c->head_stride % el == 0 && c->page_stride >= 0 && c->row_stride > 0 &&
+    VOX_REQUIRE(c->page_stride % el == 0 && c->row_stride % el == 0 && c->head_stride % el == 0 && c->page_stride > 0 && c->row_stride > 0 &&
                     c->head_stride > 0,
                 std::string(name) + ": cache strides must be positive multiples of 16 bytes");
     VOX_REQUIRE(b->seqs >= 0 && b->tokens >= 0 && b->table_width >= 0 && b->table_stride >= b->table_width && b->max_q >= 0 && b->max_kv >= 0,

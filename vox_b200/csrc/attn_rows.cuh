@@ -393,18 +393,13 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const _
             const float *po;
             slot(warp + (base + min(lane, cnt - 1)) * WPR, ml, po);
             const float2 v = lane < cnt ? __ldcg(ml) : make_float2(-INFINITY, 0.f);
-            const float mx = fmaxf(m, warp_max(v.x)), ms = mx == -INFINITY ? 0.f : mx;
-            const float alpha = ex2_approx(m - ms), w = ex2_approx(v.x - ms);
-            m = mx;
-            l = l * alpha + warp_sum(v.x == -INFINITY ? v.y : v.y * w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= alpha;
-            constexpr int U = 8;  // parts in flight
-            for (int k = 0; k < cnt; k += U) {
-                float x[U][E];
+            constexpr int U = 8;  // parts in flight; the first of them beside the statistics
+            float x[U][E];
+            auto fetch = [&](int k) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(po), min(k + u, cnt - 1))) + lane * E;
+                    if (k + u >= cnt) continue;
                     if constexpr (E == 4) {
                         const float4 f = __ldcg(reinterpret_cast<const float4 *>(src));
                         x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
@@ -413,6 +408,16 @@ __global__ void __launch_bounds__(kRowsThreads) attn_stream_merge_kernel(const _
                         x[u][0] = f.x, x[u][1] = f.y;
                     }
                 }
+            };
+            fetch(0);
+            const float mx = fmaxf(m, warp_max(v.x)), ms = mx == -INFINITY ? 0.f : mx;
+            const float alpha = ex2_approx(m - ms), w = ex2_approx(v.x - ms);
+            m = mx;
+            l = l * alpha + warp_sum(v.x == -INFINITY ? v.y : v.y * w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= alpha;
+            for (int k = 0; k < cnt; k += U) {
+                if (k > 0) fetch(k);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const float wu = __shfl_sync(0xffffffffu, w, min(k + u, 31));

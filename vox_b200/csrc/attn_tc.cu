@@ -32,7 +32,7 @@ constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 
 constexpr int POLY = 0x11;  // which of eight pairs of weights take ex2_poly
 
-constexpr int tc_stages(int hd) { return hd == 128 ? 5 : 8; }
+constexpr int tc_stages(int hd) { return hd == 128 ? 4 : 8; }
 constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }
 
 // The products of one tile, issued by one elected lane of a converged warp in one piece of code (the issuing warp runs once

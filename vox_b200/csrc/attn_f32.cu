@@ -24,7 +24,7 @@ template <typename CT, int HD> struct Tile {
 };
 
 // x = hi + lo: hi rounded to TF32's 11 significant bits in the integer unit (the conversion instruction goes through the
-// special-function unit, 16 a clock an SM, and bound the kernel: 144 us against 117 at 5 ragged prompts of 90-700 tokens, same box), lo
+// special-function unit, 16 a clock an SM: 144 us against 117 at 5 ragged prompts of 90-700 tokens, 16 heads of 64, same box), lo
 // exact in f32; the tensor cores read its first 11 bits, so hi + lo hold x to 2^-21. NaN and infinities pass through hi.
 __device__ __forceinline__ void cut(float x, uint32_t &hi, uint32_t &lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
@@ -54,7 +54,7 @@ __device__ __forceinline__ float4 load_q4(const __nv_bfloat16 *p) {
 }
 
 template <typename QT, typename CT, int HD>
-__global__ void __launch_bounds__(kRowsThreads, HD == 64 ? 3 : 2) attn_f32_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, 2) attn_f32_kernel(const __grid_constant__ AttnArgs a) {
     using T = Tile<CT, HD>;
     constexpr bool CUT = sizeof(CT) == 4;  // keys and values have a lo part
     constexpr int QC = HD / 16;            // chunks of four elements a lane takes of a row of Q and of K
@@ -138,11 +138,13 @@ __global__ void __launch_bounds__(kRowsThreads, HD == 64 ? 3 : 2) attn_f32_kerne
             if (base < whi && base + kTileKeys > wlo) {
                 const uint32_t tK = base_s + uint32_t(buf) * T::kBytes + g * T::kK + t * (4 * int(sizeof(CT)));
                 const uint32_t tV = base_s + uint32_t(buf) * T::kBytes + kTileKeys * T::kK + 2 * t * T::kV + g * (4 * int(sizeof(CT)));
-                float s[4][4];  // key tile n: rows g (registers 0-1) and g + 8, keys 8 n + 2 t, + 1
+                // key tile n: rows g (registers 0-1) and g + 8, keys 8 n + 2 t, + 1. The lo products have sums of their own: the tensor
+                // cores truncate at every step of a chain, which costs nothing at their size and a third of the steps at hi hi's
+                float s[4][4], small[4][4];
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
+                    for (int x = 0; x < 4; ++x) s[n][x] = small[n][x] = 0.f;
 #pragma unroll
                 for (int c = 0; c < QC; ++c) {
                     float k4[4][4], q0[4], q1[4];
@@ -174,14 +176,18 @@ __global__ void __launch_bounds__(kRowsThreads, HD == 64 ? 3 : 2) attn_f32_kerne
                                     bh[n][y] = __float_as_uint(k4[n][2 * h + y]);
                             }
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) mma1688(s[n], al, bh[n][0], bh[n][1]);
+                        for (int n = 0; n < 4; ++n) mma1688(small[n], al, bh[n][0], bh[n][1]);
                         if constexpr (CUT)
 #pragma unroll
-                            for (int n = 0; n < 4; ++n) mma1688(s[n], ah, bl[n][0], bl[n][1]);
+                            for (int n = 0; n < 4; ++n) mma1688(small[n], ah, bl[n][0], bl[n][1]);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) mma1688(s[n], ah, bh[n][0], bh[n][1]);
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[n][x] += small[n][x];
                 if (base < all_lo || base + kTileKeys > all_hi) {
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
@@ -226,11 +232,11 @@ __global__ void __launch_bounds__(kRowsThreads, HD == 64 ? 3 : 2) attn_f32_kerne
                 }
 #pragma unroll
                 for (int c = 0; c < VC; ++c) {
-                    float d[4][4];
+                    float d[4][4], ds[4][4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) d[e][x] = 0.f;
+                        for (int x = 0; x < 4; ++x) d[e][x] = ds[e][x] = 0.f;
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
                         float v0[4], v1[4];
@@ -247,17 +253,17 @@ __global__ void __launch_bounds__(kRowsThreads, HD == 64 ? 3 : 2) attn_f32_kerne
                             }
                         }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mma1688(d[e], pl[n], bh[e][0], bh[e][1]);
+                        for (int e = 0; e < 4; ++e) mma1688(ds[e], pl[n], bh[e][0], bh[e][1]);
                         if constexpr (CUT)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) mma1688(d[e], ph[n], bl[e][0], bl[e][1]);
+                            for (int e = 0; e < 4; ++e) mma1688(ds[e], ph[n], bl[e][0], bl[e][1]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) mma1688(d[e], ph[n], bh[e][0], bh[e][1]);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[c][e][x] += d[e][x];
+                        for (int x = 0; x < 4; ++x) acc[c][e][x] += d[e][x] + ds[e][x];
                 }
             }
             __syncthreads();  // the buffer is filled again two tiles on

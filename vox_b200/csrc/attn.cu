@@ -1,5 +1,6 @@
 // Attention over a paged key/value cache: vox_cuda_attn_paged and vox_cuda_attn_prefix, their split of the work, the
 // CUDA-core kernel (f32 caches) and the join of split rows.
+#include <algorithm>
 #include <cmath>
 
 #include "attn_rows.cuh"
@@ -15,7 +16,8 @@ __device__ __forceinline__ float load_f(const __nv_bfloat16 *p) { return __bfloa
 // bytes, so a warp load brings KPW keys; each group of LPK lanes keeps its own running maximum, sum and output of every
 // row, so the loop over the keys has no exchange between groups: per key and row one dot product (a butterfly over the LPK
 // lanes), one 2^x, and one multiply-add per element of v. Every warp takes each kRowsWarps-th run of KPI keys, U loads of K
-// and U of V in flight before the first is used. The groups of a warp are joined at the end.
+// and U of V in flight before the first is used. The groups of a warp are joined at the end. Bound by latency: one token of
+// 16 query heads on 8 of 128 at 650 keys takes 8.7 us in a graph, of which the 5 MB would need 0.8.
 template <typename QT, int HD_, int R>
 struct VecCore {
     using Q = QT;
@@ -27,7 +29,6 @@ struct VecCore {
         __shared__ float s_acc[kRowsWarps][RB][HD];
         return s_acc;
     }
-
 
     template <typename F>
     static __device__ __forceinline__ void run(const AttnArgs &a, const RowsJob &j, float (*s_acc)[RB][HD], float2 (*s_ml)[RB], State &, F between) {
@@ -212,18 +213,26 @@ void cut_keys(int64_t keys, int64_t want, int &splits, int &chunk) {
     chunk = int(per * 128);
 }
 
+//
+// Times beside a rule: of a 16-head call on 8 key/value heads of 128, in a graph, by the rule and by the other side.
 AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cache, int64_t max_q, int64_t max_kv, int64_t prefix_len) {
     AttnShape s = {};
     const int64_t rows = max_q * p.group, all = int64_t(p.tokens) * p.group, sms = sm_count(), base = int64_t(p.seqs) * p.kv_heads;
     const bool f32 = dtype == VOX_CUDA_F32, tc_types = !f32 && bf16_cache;
     s.mma = bf16_cache;
     s.rows_blk = s.mma ? (rows <= 8 || f32 ? 8 : 16) : rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
-    s.wide = !tc_types && rows > 16;
+    // f32 accuracy by TF32 in 64-row blocks, above as many rows as the few-row kernels read the keys for at once or nearly so: f32
+    // caches, 8 sequences of 1000 keys, 8 rows 34.5 us (42 wide), 12 rows 42.9 wide (66.2); bf16 caches, which the few-row
+    // kernel takes 8 rows a block from the tensor cores, 32 rows 31.8 us (39.1 wide), 64 rows 44 wide (50)
+    s.wide = !tc_types && rows > (bf16_cache ? 32 : 8);
     if (s.wide) s.rows_blk = kF32Rows;
     s.pre_wide = !tc_types && !s.wide && all >= 2 * kF32Rows;
+    // 16 sequences of 2000 keys: 16 rows 33 us (38 on attn_tc.cu), 24 rows 37.6 there (57)
     s.own_tc = tc_types && rows > 16;
     s.pre_tc = tc_types && all > 16;
-    s.concat = prefix_len > 0 && s.own_tc && rows >= 64;
+    // 24 texts behind 1003 shared rows: the prefix in front of each text's own keys, without a join, 128 rows a text 37.4 us
+    // (48.5 apart), up to 300 rows 52 (55); 64 rows 38.0 apart (41)
+    s.concat = prefix_len > 0 && s.own_tc && rows > 64;
     if (prefix_len > 0 && !s.concat) {
         const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.pre_wide ? kF32Rows : s.rows_blk;
         if (s.pre_tc) s.tc_rows = rb;
@@ -233,16 +242,21 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         s.pre_blocks = pre * s.pre_splits;
     }
     if (s.own_tc) {
-        // row tiles of all sequences together: exact for equal counts, else one more a sequence at most
-        auto tiles = [&](int64_t rb) { return p.q_start ? all / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
+        // row tiles of all sequences together: no more than `bound` (the launch covers it), and `tiles` where max_q holds
+        auto bound = [&](int64_t rb) { return p.q_start ? (all - p.seqs) / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
+        auto tiles = [&](int64_t rb) { return std::max<int64_t>(std::min(bound(rb), p.seqs * ((rows + rb - 1) / rb)), 1); };
+        // both row tiles of a block on different rows halve the reads of keys and fill its softmax's gaps, but halve the blocks:
+        // one prompt of 300 tokens 12.6 us with 128 rows a block (14.4 with 256), of 1000 20.2 (23.0); 24 texts of 7-150 tokens
+        // behind 1003 rows 52 with 256 (63)
         if (s.tc_rows == 0) s.tc_rows = tiles(256) * p.kv_heads >= sms / 2 ? 256 : 128;
-        s.own_tiles = int(tiles(s.tc_rows));
-        const int64_t own = int64_t(s.own_tiles) * p.kv_heads;
-        cut_keys(max_kv, s.concat ? 1 : own < sms ? sms / own : 1, s.own_splits, s.own_chunk);
-        s.own_units = own * s.own_splits;
+        s.own_tiles = int(bound(s.tc_rows));
+        const int64_t busy = tiles(s.tc_rows) * p.kv_heads;
+        cut_keys(max_kv, s.concat ? 1 : busy < sms ? sms / busy : 1, s.own_splits, s.own_chunk);
+        s.own_units = int64_t(s.own_tiles) * p.kv_heads * s.own_splits;
     } else if (!s.wide && rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc || s.pre_wide) && base * ((int64_t(p.cap) >> 6) + 1) < (int64_t(1) << 31)) {
         // one row tile a sequence: a cluster for each sequence and key/value head where one wave of blocks holds them all
-        // with at most 512 keys each, else equal runs of all sequences' tiles
+        // with at most 512 keys each, else equal runs of all sequences' tiles: 8 sequences of 1000-2000 keys 12.4 us in clusters
+        // (14.1 in runs), 30 of up to 500 5.8 (7.3); one of 8192 keys 13.7 in runs (18.2), of 16384 16.3 (30.6)
         const int64_t resident = s.mma ? attn_mma_resident(head_dim, s.rows_blk, dtype)
                                        : with_vec(dtype, head_dim, s.rows_blk, [](auto core) { return rows_resident<decltype(core)>(); });
         int c = 8;

@@ -8,6 +8,13 @@
 //   layout if V's rows are taken in that order, and V's chunks of four elements serve four column tiles, so nothing is
 //   shuffled. Each tile's P V is added to the running output by f32 additions (the tensor cores' own accumulation truncates).
 // Row strides in shared memory are padded so that the eight lanes of a 16-byte access phase hit different banks.
+//
+// The tensor cores' truncation bends f32 results, so chains of products stay short and the small lo products, which one
+// truncation at the size of the hi sum would swallow, have sums of their own: largest error against 64 bits 5.0e-7 of the
+// output's scale, as against 1.1e-6 in one sum (sums in f32 by plain matrix products: 6.3e-7).
+// Bound by the issue and latency of the products (three mma of 16 x 8 x 8 a step, and the cutting of operands between), not by
+// bytes: 5 ragged prompts of 90-700 tokens, 16 heads of 64, take 113 us where their bytes would need 6. Two blocks an SM
+// (at most 255 registers, nothing spilled) 113 us against 125 with one and 117 with operands that spill.
 #include "attn_rows.cuh"
 
 namespace voxcuda {

@@ -13,7 +13,8 @@
 //                        (sequence, then key/value head, then tile), whatever their lengths: the lengths are on the device,
 //                        so the host cannot balance them. A block that covers a sequence's keys whole stores its rows;
 //                        the others leave at most two parts a block (the end of one sequence, the start of another), which
-//                        attn_stream_merge_kernel joins in ascending order of keys.
+//                        attn_stream_merge_kernel joins in ascending order of keys. The joining launch costs
+//                        some 5 us, most of it its start and the parts' way through L2; attn.cu has when it pays.
 #pragma once
 
 #include "attn.cuh"

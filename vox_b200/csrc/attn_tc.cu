@@ -13,6 +13,12 @@
 //                   page); rows of V past the last key are zeroed (their weight is 0, and 0 times what lies there may be NaN)
 //   warps 9, 10     issue the products of row tile 0, 1: P V of a step, then Q K^T two steps on into the same S buffer
 // Tile order in the ring: K0 V0 K1 V1 ... (both row tiles read each). Every wait is bounded.
+//
+// Measured: one prompt of 8192 tokens, 16 query heads on 8 of 128, 231 us in a graph: 1190 TFLOP/s of the causal half, 0.71 of
+// what a bare product reaches. Bound by the softmax, some 1610 clocks per 64 keys of both row tiles (exponentials, their
+// latency, and the tensor-memory loads before them) where the products need half; every block adds some 6 us before its
+// first and after its last product. One S buffer a row tile and steps of 128 keys, so that the products stand in the softmax's
+// path: 249 us against 210 at 7 ragged prompts, 56 against 50 at 24 texts behind one prefix.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -30,7 +36,9 @@ constexpr int kStepKeys = 64;
 constexpr int kTcThreads = 352;
 constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 
-constexpr int POLY = 0x11;  // which of eight pairs of weights take ex2_poly
+// Which of eight pairs of weights take ex2_poly. 1, 2, 3 or 4 of them: 230.6, 231.3, 238, 247 us at one prompt of 8192 tokens
+// and 68.1, 66.7, 67.4, 69.9 at 4096.
+constexpr int POLY = 0x11;
 
 constexpr int tc_stages(int hd) { return hd == 128 ? 4 : 8; }
 constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }

@@ -230,9 +230,15 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
     // 16 sequences of 2000 keys: 16 rows 33 us (38 on attn_tc.cu), 24 rows 37.6 there (57)
     s.own_tc = tc_types && rows > 16;
     s.pre_tc = tc_types && all > 16;
-    // 24 texts behind 1003 shared rows: the prefix in front of each text's own keys, without a join, 128 rows a text 37.4 us
-    // (48.5 apart), up to 300 rows 52 (55); 64 rows 38.0 apart (41)
-    s.concat = prefix_len > 0 && s.own_tc && rows > 64;
+    // row tiles of all sequences together: no more than `bound` (the launch covers it), and `tiles` where max_q holds
+    auto bound = [&](int64_t rb) { return p.q_start ? (all - p.seqs) / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
+    auto tiles = [&](int64_t rb) { return std::max<int64_t>(std::min(bound(rb), p.seqs * ((rows + rb - 1) / rb)), 1); };
+    // The prefix in front of each text's own keys in the same block, without a join; or apart, for the rows of all texts
+    // together, which fill their row tiles: apart if that spares an SM more than ten tiles of 128 keys, or the texts are short.
+    // 24 texts behind 1003 rows: 128 rows a text 37.2 us (38.9 apart), 200 rows 54.9 (57.9), 14-300 rows 52 (50.7), 64 rows 36.2
+    // apart (41); 64 texts of 14-200 rows behind 4000 161 apart (284), 8 of 60-600 82.7 (84.7)
+    s.concat = prefix_len > 0 && s.own_tc && rows > 64 &&
+               (tiles(256) - ceil_div(all, 256)) * p.kv_heads * prefix_len <= int64_t(10) * 128 * sms;
     if (prefix_len > 0 && !s.concat) {
         const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.pre_wide ? kF32Rows : s.rows_blk;
         if (s.pre_tc) s.tc_rows = rb;
@@ -242,9 +248,6 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         s.pre_blocks = pre * s.pre_splits;
     }
     if (s.own_tc) {
-        // row tiles of all sequences together: no more than `bound` (the launch covers it), and `tiles` where max_q holds
-        auto bound = [&](int64_t rb) { return p.q_start ? (all - p.seqs) / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
-        auto tiles = [&](int64_t rb) { return std::max<int64_t>(std::min(bound(rb), p.seqs * ((rows + rb - 1) / rb)), 1); };
         // both row tiles of a block on different rows halve the reads of keys and fill its softmax's gaps, but halve the blocks:
         // one prompt of 300 tokens 12.6 us with 128 rows a block (14.4 with 256), of 1000 20.2 (23.0); 24 texts of 7-150 tokens
         // behind 1003 rows 52 with 256 (63)
@@ -363,22 +366,16 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     using bf = __nv_bfloat16;
     const bool qf = dtype == VOX_CUDA_F32;
     int r = VOX_CUDA_OK;
-    if (s.pre_blocks > 0 && s.pre_tc) {
-        a.tc_prefix = 1;
-        r = attn_tc_launch(a, *cache, s.pre_blocks, st, name);
-        a.tc_prefix = 0;
-        if (r != VOX_CUDA_OK) return r;
-    }
-    if (s.pre_blocks > 0 && s.pre_wide) {
+    if (s.pre_blocks > 0 && (s.pre_wide || (s.pre_tc && !s.own_tc))) {  // the prefix in a launch of its own
         a.pre_blocks = int32_t(s.pre_blocks);
-        r = attn_f32_launch(a, hd, dtype, cache->dtype, s.pre_blocks, st, name);
+        r = s.pre_tc ? attn_tc_launch(a, *cache, s.pre_blocks, st, name) : attn_f32_launch(a, hd, dtype, cache->dtype, s.pre_blocks, st, name);
         if (r != VOX_CUDA_OK) return r;
     }
+    a.pre_blocks = s.pre_wide || (s.pre_tc && !s.own_tc) ? 0 : int32_t(s.pre_blocks);
+    const int64_t n = a.pre_blocks + s.own_units;
     if (s.own_tc) {
-        r = attn_tc_launch(a, *cache, s.own_units, st, name);
+        r = attn_tc_launch(a, *cache, n, st, name);
     } else {
-        a.pre_blocks = s.pre_tc || s.pre_wide ? 0 : int32_t(s.pre_blocks);
-        const int64_t n = a.pre_blocks + s.own_units;
         if (s.wide) {
             r = attn_f32_launch(a, hd, dtype, cache->dtype, n, st, name);
         } else if (s.mma) {

@@ -32,7 +32,7 @@ struct AttnArgs {
     int32_t partial;                           // results go to the workspace (a row's parts meet in a later launch)
     // the tensor-core kernel: rows a block; whether this launch takes the prefix; whether the own keys follow the prefix
     // in one walk (then pre_splits is 0). own_tiles counts the row tiles of all sequences there.
-    int32_t tc_rows, tc_prefix, concat;
+    int32_t tc_rows, concat;
     // there the scale is positive (row maxima are taken before it): a negative one flips q's signs, zero clears q
     float tc_scale;
     uint32_t q_and, q_xor;

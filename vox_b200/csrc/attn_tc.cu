@@ -111,9 +111,11 @@ struct TcJob {
 __device__ __forceinline__ void tc_job(const AttnArgs &a, uint32_t blk, TcJob &out) {
     const int lane = threadIdx.x & 31;
     TcJob j = {};
+    const bool prefix = blk < uint32_t(a.pre_blocks);
+    if (!prefix) blk -= uint32_t(a.pre_blocks);
     uint32_t y = a.kvdiv.div(blk);
     j.kvh = int(blk - y * uint32_t(a.p.kv_heads));
-    if (a.tc_prefix) {  // rows of all tokens against a split of the prefix
+    if (prefix) {  // rows of all tokens against a split of the prefix
         const uint32_t s = a.ptdiv.div(y);
         j.row0 = int(y - s * uint32_t(a.pre_tiles)) * a.tc_rows;
         j.rows = a.p.tokens * a.p.group;

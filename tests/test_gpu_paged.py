@@ -544,6 +544,58 @@ def test_prefix_of_many_tiles(vox, act, cache, q):
 
 
 @pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("heads,kvh,hd", [(16, 8, 128), (14, 2, 64)])
+@pytest.mark.parametrize("prefix", [1, 17, 300, 1500])
+def test_prefix_of_few_short_sequences(vox, act, cache, heads, kvh, hd, prefix):
+    """Single tokens of few sequences, so that a call's blocks take the prefix and the own rows side by side: prefixes of one
+    row to several blocks, own rows of one to more than max_kv said, a sequence without new tokens."""
+    bt = Batch([(1, 1), (1, 130), (0, 9), (1, 511), (1, 16)], kvh, hd, 16, cache, seed=prefix, prefix=prefix)
+    q = queries(bt, heads, act)
+    table, kv_len, q_start = bt.dev()
+    want, mag, big = attention64(bt, q, heads, hd ** -0.5)
+    h, pre = bt.handle(vox), bt.prefix_pages.cuda()
+    for max_kv in (511, 40, 0):
+        got = h.attend_prefix(q.cuda(), pre, prefix, table, kv_len, q_start=q_start, max_q=1, max_kv=max_kv)
+        check(got, want, mag, big, act, cache, 2100)
+        assert torch.equal(got, h.attend_prefix(q.cuda(), pre, prefix, table, kv_len, q_start=q_start, max_q=1, max_kv=max_kv))
+    assert vox.device_error() == 0
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("seqs,longest,prefix", [(24, 4, 700), (48, 36, 1000)])
+def test_prefix_of_many_texts(vox, act, cache, seqs, longest, prefix):
+    """Texts that fill little of a row tile each behind a long prefix, counted together and apart."""
+    r = np.random.default_rng(seqs)
+    lens = [(int(n), int(n) + int(e)) for n, e in zip(r.integers(1, longest + 1, seqs), r.integers(0, 30, seqs))]
+    lens[3], lens[7] = (longest, longest), (0, 5)
+    bt = Batch(lens, 8, 64, 16, cache, seed=seqs, prefix=prefix)
+    q = queries(bt, 56, act)
+    table, kv_len, q_start = bt.dev()
+    want, mag, big = attention64(bt, q, 56, 64 ** -0.5)
+    h = bt.handle(vox)
+    for mq, mkv in ((longest, longest + 30), (1, 1), (0, 0)):
+        got = h.attend_prefix(q.cuda(), bt.prefix_pages.cuda(), prefix, table, kv_len, q_start=q_start, max_q=mq, max_kv=mkv)
+        check(got, want, mag, big, act, cache, prefix + longest + 30)
+    assert vox.device_error() == 0
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("q", [4, 5, 8, 9, 16, 17])
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_rows_where_the_kernels_change(vox, act, cache, q, prefix):
+    """Two query heads a key/value head: 8, 10, 16, 18, 32 and 34 rows a sequence."""
+    bt = Batch([(q, q), (q, 150), (q, q + 1), (q, 333), (q, 0), (q, 2)], 2, 128, 32, cache, seed=q, prefix=prefix)
+    x = queries(bt, 4, act)
+    table, kv_len, _ = bt.dev(uniform=True)
+    h = bt.handle(vox)
+    got = h.attend_prefix(x.cuda(), bt.prefix_pages.cuda(), prefix, table, kv_len, max_kv=333) if prefix else \
+        h.attend(x.cuda(), table, kv_len, max_kv=333)
+    want, mag, big = attention64(bt, x, 4, 128 ** -0.5)
+    check(got, want, mag, big, act, cache, 540)
+    assert vox.device_error() == 0
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
 def test_scores_that_keep_rising(vox, act, cache):
     """Every step's largest score is far above the last one's, so the running maximum moves at each; and far below, so it
     never does."""

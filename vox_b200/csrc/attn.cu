@@ -199,7 +199,7 @@ struct AttnShape {
     int rows_blk, tc_rows;
     int own_tiles, own_splits, own_chunk;
     int pre_tiles, pre_splits, pre_chunk;
-    int cluster, stream_shift, stream_rows;
+    int cluster, cluster_pre, stream_shift, stream_rows;
     int64_t own_units, pre_blocks;     // blocks, or clusters
     int slots;                         // of a row in the workspace
 };
@@ -239,6 +239,24 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
     // apart (41); 64 texts of 14-200 rows behind 4000 161 apart (284), 8 of 60-600 82.7 (84.7)
     s.concat = prefix_len > 0 && s.own_tc && rows > 64 &&
                (tiles(256) - ceil_div(all, 256)) * p.kv_heads * prefix_len <= int64_t(10) * 128 * sms;
+    // one row tile a sequence?
+    const bool one_tile = !s.own_tc && !s.wide && rows <= s.rows_blk;
+    const int64_t resident = !one_tile ? 0
+                             : s.mma   ? attn_mma_resident(head_dim, s.rows_blk, dtype)
+                                       : with_vec(dtype, head_dim, s.rows_blk, [](auto core) { return rows_resident<decltype(core)>(); });
+    if (prefix_len > 0 && one_tile) {
+        // one launch of clusters that take the prefix too, by the same rule as below: 8 sequences of up to 1000 rows behind 1003
+        // 12.6 us (17.7 in launches apart), 14 heads on 2 of 64 7.9 (14.2)
+        int c = 8;
+        while (c > 2 && (base * c > resident || 32 * c > prefix_len + max_kv)) c /= 2;
+        const int64_t cp = std::clamp<int64_t>((c * prefix_len + (prefix_len + max_kv) / 2) / (prefix_len + max_kv), 1, c - 1);
+        if (base * c <= resident && prefix_len <= 512 * cp && max_kv <= 512 * (c - cp)) {
+            s.frame = kFrameCluster;
+            s.cluster = c, s.cluster_pre = int(cp);
+            s.own_units = base;
+            return s;
+        }
+    }
     if (prefix_len > 0 && !s.concat) {
         const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.pre_wide ? kF32Rows : s.rows_blk;
         if (s.pre_tc) s.tc_rows = rb;
@@ -256,12 +274,10 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         const int64_t busy = tiles(s.tc_rows) * p.kv_heads;
         cut_keys(max_kv, s.concat ? 1 : busy < sms ? sms / busy : 1, s.own_splits, s.own_chunk);
         s.own_units = int64_t(s.own_tiles) * p.kv_heads * s.own_splits;
-    } else if (!s.wide && rows <= s.rows_blk && (prefix_len == 0 || s.pre_tc || s.pre_wide) && base * ((int64_t(p.cap) >> 6) + 1) < (int64_t(1) << 31)) {
+    } else if (one_tile && (prefix_len == 0 || s.pre_tc || s.pre_wide) && base * ((int64_t(p.cap) >> 6) + 1) < (int64_t(1) << 31)) {
         // one row tile a sequence: a cluster for each sequence and key/value head where one wave of blocks holds them all
         // with at most 512 keys each, else equal runs of all sequences' tiles: 8 sequences of 1000-2000 keys 12.4 us in clusters
         // (14.1 in runs), 30 of up to 500 5.8 (7.3); one of 8192 keys 13.7 in runs (18.2), of 16384 16.3 (30.6)
-        const int64_t resident = s.mma ? attn_mma_resident(head_dim, s.rows_blk, dtype)
-                                       : with_vec(dtype, head_dim, s.rows_blk, [](auto core) { return rows_resident<decltype(core)>(); });
         int c = 8;
         while (c > 1 && (base * c > resident || 32 * c > max_kv)) c /= 2;
         if (base * c <= resident && max_kv <= 512 * c) {
@@ -356,7 +372,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
     a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;
     a.tc_rows = s.tc_rows, a.concat = s.concat;
-    a.cluster = s.cluster, a.stream_shift = s.stream_shift, a.stream_rows = s.stream_rows, a.stream_rb = s.rows_blk;
+    a.cluster = s.cluster, a.cluster_pre = s.cluster_pre, a.stream_shift = s.stream_shift, a.stream_rows = s.stream_rows, a.stream_rb = s.rows_blk;
     a.stream_blocks = int32_t(s.frame == kFrameStream ? s.own_units : 0);
     char *scratch = static_cast<char *>(workspace);
     a.part_o = reinterpret_cast<float *>(scratch), a.part_ml = reinterpret_cast<float2 *>(scratch + w.part_ml);

@@ -36,9 +36,9 @@ struct AttnArgs {
     // there the scale is positive (row maxima are taken before it): a negative one flips q's signs, zero clears q
     float tc_scale;
     uint32_t q_and, q_xor;
-    // few query rows (attn_rows.cuh): blocks a cluster; or log2 of the keys a tile of the list, rows that the joining launch looks at,
+    // few query rows (attn_rows.cuh): blocks a cluster and how many of them take the prefix; or log2 of the keys a tile of the list, rows that the joining launch looks at,
     // rows and number of the parts, and the parts themselves
-    int32_t cluster, stream_shift, stream_rows, stream_rb, stream_blocks;
+    int32_t cluster, cluster_pre, stream_shift, stream_rows, stream_rb, stream_blocks;
     float *stream_o;
     float2 *stream_ml;
     CUtensorMap mk, mv;  // the cache's tensors, boxes of 16 rows of one page (attn_mma.cu)

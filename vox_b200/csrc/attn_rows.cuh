@@ -149,7 +149,9 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
     return v;
 }
 
-// Grid: clusters of a.cluster blocks; cluster c takes key/value head c % kv_heads of sequence c / kv_heads.
+// Grid: clusters of a.cluster blocks; cluster c takes key/value head c % kv_heads of sequence c / kv_heads. The first
+// a.cluster_pre blocks of each take the shared prefix, where a call is so small that its launches cost more than reading the
+// prefix again for every sequence.
 template <class Core>
 __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
@@ -164,13 +166,15 @@ __global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_cluster_k
     int tok0, n;
     seq_tokens(a.p, int(b), tok0, n);
     const int kv = seq_rows(a.p, int(b)), rows = n * a.p.group;
+    const bool pre = int(rank) < a.cluster_pre;
+    const int keys = pre ? a.prefix_len : kv, blocks = pre ? a.cluster_pre : a.cluster - a.cluster_pre;
     int lo = 0;
-    if (a.window > 0) lo = max(kv - n + 1 - a.window, 0) & ~15;
-    const int per = ((kv - lo + a.cluster - 1) / a.cluster + 15) & ~15;
-    const int k0 = min(lo + int(rank) * per, kv), k1 = min(k0 + per, kv);
-    const int32_t *pages = a.p.table + int64_t(b) * a.p.table_stride;
+    if (a.window > 0) lo = max(kv - n + 1 - a.window, 0) & ~15;  // there is no prefix then
+    const int per = ((keys - lo + blocks - 1) / blocks + 15) & ~15;
+    const int k0 = min(lo + (pre ? int(rank) : int(rank) - a.cluster_pre) * per, keys), k1 = min(k0 + per, keys);
+    const int32_t *pages = pre ? a.prefix_pages : a.p.table + int64_t(b) * a.p.table_stride;
     for (int row0 = 0; row0 < rows; row0 += RB) {  // the same rows in every block of the cluster
-        Core::run(a, RowsJob{tok0, rows, row0, kvh, kv - n, true, k0, k1, pages}, s_acc, s_ml, core, [] {});
+        Core::run(a, RowsJob{tok0, rows, row0, kvh, kv - n, !pre, k0, k1, pages}, s_acc, s_ml, core, [] {});
         __syncthreads();
         Join mine[(RB * (HD / 4) + kRowsThreads - 1) / kRowsThreads];
 #pragma unroll

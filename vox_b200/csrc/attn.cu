@@ -11,13 +11,36 @@ namespace {
 __device__ __forceinline__ float load_f(const float *p) { return *p; }
 __device__ __forceinline__ float load_f(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 
+// Sums c values over 2 o lanes, each lane left with c / (2 o) whole sums (at least one): at every exchange a lane gives half of its
+// values away and adds what it gets to the other half, the upper for the upper lane.
+template <int O, int CNT, int N>
+__device__ __forceinline__ void halve(float (&s)[N], int lane) {
+    if constexpr (O > 0) {
+        constexpr int H = CNT > 1 ? CNT / 2 : 1;
+        if constexpr (CNT > 1) {
+            const bool up = lane & O;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                const float give = up ? s[i] : s[i + H], keep = up ? s[i + H] : s[i];
+                s[i] = keep + __shfl_xor_sync(0xffffffffu, give, O);
+            }
+        } else {
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], O);
+        }
+        halve<O / 2, H>(s, lane);
+    }
+}
+
 // softmax(scale q k^T) v on the CUDA cores for an f32 cache, f32 throughout: R rows (query heads that share a key/value
 // head, of one or more tokens) against a range of keys. Lane layout: a key's row of HD elements takes LPK lanes of 16
-// bytes, so a warp load brings KPW keys; each group of LPK lanes keeps its own running maximum, sum and output of every
-// row, so the loop over the keys has no exchange between groups: per key and row one dot product (a butterfly over the LPK
-// lanes), one 2^x, and one multiply-add per element of v. Every warp takes each kRowsWarps-th run of KPI keys, U loads of K
-// and U of V in flight before the first is used. The groups of a warp are joined at the end. Bound by latency: one token of
-// 16 query heads on 8 of 128 at 650 keys takes 8.7 us in a graph, of which the 5 MB would need 0.8.
+// bytes, so a warp load brings KPW keys (one a group of LPK lanes); a step takes U of them. The U R dot products of a step are
+// summed over the group by halving: a lane gives half of its values away at each exchange and adds what it gets to the
+// other half, so it ends with the whole sum of one (row, key) pair (or C of them, or D lanes with the same one), takes its
+// 2^x alone, keeps the sum of its weights, and hands the weights to the group through shared memory. That is about one exchange a
+// score. (A butterfly for each, every lane taking every 2^x: 201 us against 139 at 32 sequences of 2000-4000 keys and 4 rows, 369
+// against 227 at 8.) The rows' references are the warp's
+// and move only when a score exceeds one by 8 (base 2): the common step has one vote. Every warp takes each kRowsWarps-th
+// run of KPI keys; from four rows on, the next step's K is loaded while this one's weights and products are worked on.
 template <typename QT, int HD_, int R>
 struct VecCore {
     using Q = QT;
@@ -37,13 +60,16 @@ struct VecCore {
         constexpr int LPK = HD / V, KPW = 32 / LPK; // lanes a key, keys a warp load
         constexpr int U = R <= 2 ? 8 : 4;           // loads of K (and of V) in flight
         constexpr int KPI = KPW * U;                // keys a step; divides or is a multiple of 16
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane / LPK, e0 = (lane % LPK) * V, row0 = j.row0;
+        constexpr int N = U * R, C = N >= LPK ? N / LPK : 1, D = N >= LPK ? 1 : LPK / N;
+        constexpr int kRowLanes = LPK / R;          // of a group
+        constexpr bool kAhead = R >= 4;
+        __shared__ __align__(16) float s_p[kRowsWarps][2][KPW][N + 4];
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane / LPK, li = lane % LPK, e0 = li * V, row0 = j.row0;
+        const int mine = li * C / D, row = mine / U, u0 = mine % U;  // this lane's scores: row `row`, keys u0 .. u0 + C - 1 of the group
         const float *K = static_cast<const float *>(a.p.k) + int64_t(j.kvh) * a.p.head_stride + e0;
         const float *Vp = static_cast<const float *>(a.p.v) + int64_t(j.kvh) * a.p.head_stride + e0;
         float2 q[R][V / 2], acc[R][V / 2];
-        float m[R], l[R];
-        int hi[R], lo[R];
-        int kmin = j.k1, kend = j.k0;
+        int kmin = j.k1, kend = j.k0, hi = 0, lo = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int rr = min(row0 + r, j.rows - 1);
@@ -54,89 +80,116 @@ struct VecCore {
                 q[r][e] = make_float2(load_f(src + 2 * e) * a.scale_log2, load_f(src + 2 * e + 1) * a.scale_log2);
                 acc[r][e] = make_float2(0.f, 0.f);
             }
-            m[r] = -INFINITY, l[r] = 0.f;
-            hi[r] = j.causal ? min(j.base + i + 1, j.k1) : j.k1;
-            lo[r] = a.window > 0 && j.causal ? max(j.base + i + 1 - a.window, j.k0) : j.k0;
-            kmin = min(kmin, lo[r]), kend = max(kend, hi[r]);
+            const int h1 = j.causal ? min(j.base + i + 1, j.k1) : j.k1;
+            const int l0 = a.window > 0 && j.causal ? max(j.base + i + 1 - a.window, j.k0) : j.k0;
+            kmin = min(kmin, l0), kend = max(kend, h1);
+            if (r == row) hi = h1, lo = l0;
         }
-        for (int base = (kmin & ~15) + warp * KPI; base < kend; base += kRowsWarps * KPI) {
-            uint4 kr[U], vr[U];
+        float m = -INFINITY, l = 0.f;  // the row's reference; this lane's weights
+        uint4 kr[U], vr[U];
+        int64_t off[U];
+        auto load_k = [&](int base) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int key = base + u * KPW + grp;
-                kr[u] = vr[u] = make_uint4(0, 0, 0, 0);  // rows outside the range are never read: zero weight times zero
+                kr[u] = make_uint4(0, 0, 0, 0), off[u] = -1;  // rows outside the range are never read: zero weight times zero
                 if (key >= kmin && key < kend) {
                     const int page = page_checked(a.p, __ldg(j.pages + (key >> a.p.page_shift)));
-                    const int64_t off = int64_t(page) * a.p.page_stride + int64_t(key & a.p.page_mask) * a.p.row_stride;
-                    kr[u] = ld_stream(K + off);
-                    vr[u] = ld_stream(Vp + off);
+                    off[u] = int64_t(page) * a.p.page_stride + int64_t(key & a.p.page_mask) * a.p.row_stride;
+                    kr[u] = ld_stream(K + off[u]);
                 }
             }
-            float s[U][R];
+        };
+        int base = (kmin & ~15) + warp * KPI, buf = 0;
+        if (kAhead && base < kend) load_k(base);
+        for (; base < kend; base += kRowsWarps * KPI, buf ^= 1) {
+            if (!kAhead) load_k(base);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                vr[u] = make_uint4(0, 0, 0, 0);
+                if (off[u] >= 0) vr[u] = ld_stream(Vp + off[u]);
+            }
+            float s[N];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float2 kf[V / 2];
                 unpack2<VOX_CUDA_F32>(kr[u], kf);
-                const int key = base + u * KPW + grp;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     float2 d = mul2(q[r][0], kf[0]);
 #pragma unroll
                     for (int e = 1; e < V / 2; ++e) d = fma2(q[r][e], kf[e], d);
-                    float x = d.x + d.y;
-#pragma unroll
-                    for (int o = LPK / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                    s[u][r] = key >= lo[r] && key < hi[r] ? x : -INFINITY;
+                    s[r * U + u] = d.x + d.y;
                 }
             }
+            if (kAhead && base + kRowsWarps * KPI < kend) load_k(base + kRowsWarps * KPI);
+            halve<LPK / 2, N>(s, lane);
+            float top = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float mx = m[r];
+            for (int i = 0; i < C; ++i) {
+                const int key = base + (u0 + i) * KPW + grp;
+                if (key < lo || key >= hi) s[i] = -INFINITY;
+                top = fmaxf(top, s[i]);
+            }
+            if (__any_sync(0xffffffffu, top > m + 8.f)) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u][r]);
-                const float ms = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: every weight below is 2^-inf = 0
-                const float alpha = ex2_approx(m[r] - ms);
-                m[r] = mx;
-                l[r] *= alpha;
+                for (int o = 1; o < kRowLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    s[u][r] = ex2_approx(s[u][r] - ms);
-                    l[r] += s[u][r];
+                for (int o = LPK; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = fmaxf(top, m);
+                const float alpha = ex2_approx(m - (top == -INFINITY ? 0.f : top));  // nothing seen before: 0
+                m = top;
+                l *= alpha;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float w = __shfl_sync(0xffffffffu, alpha, r * kRowLanes);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) acc[r][e] = mul2(acc[r][e], bc2(w));
                 }
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) acc[r][e] = mul2(acc[r][e], bc2(alpha));
             }
+            const float ref = m == -INFINITY ? 0.f : m;  // nothing seen yet: the weights are 2^-inf = 0
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float2 vf[V / 2];
-                unpack2<VOX_CUDA_F32>(vr[u], vf);
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int e = 0; e < V / 2; ++e) acc[r][e] = fma2(vf[e], bc2(s[u][r]), acc[r][e]);
+            for (int i = 0; i < C; ++i) {
+                const float p = ex2_approx(s[i] - ref);
+                l += p;
+                if (D == 1 || li % D == 0) s_p[warp][buf][grp][mine + i] = p;
             }
+            __syncwarp();  // the other buffer's readers are past the last one
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int u = 0; u < U; u += 4) {
+                    const float4 p = *reinterpret_cast<const float4 *>(&s_p[warp][buf][grp][r * U + u]);
+                    const float w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float2 vf[V / 2];
+                        unpack2<VOX_CUDA_F32>(vr[u + k], vf);
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) acc[r][e] = fma2(vf[e], bc2(w[k]), acc[r][e]);
+                    }
+                }
         }
-        // the lane groups of a warp, then the warps
+        if (D > 1 && li % D != 0) l = 0.f;  // counted by the lane's twin
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int o = 1; o < kRowLanes; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-            for (int o = LPK; o < 32; o <<= 1) {
-                const float mo = __shfl_xor_sync(0xffffffffu, m[r], o), lo2 = __shfl_xor_sync(0xffffffffu, l[r], o);
-                const float mx = fmaxf(m[r], mo), ms = mx == -INFINITY ? 0.f : mx;
-                const float wa = ex2_approx(m[r] - ms), wb = ex2_approx(mo - ms);
-                m[r] = mx;
-                l[r] = l[r] * wa + lo2 * wb;
+        for (int o = LPK; o < 32; o <<= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
-                    const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, acc[r][e].x, o), __shfl_xor_sync(0xffffffffu, acc[r][e].y, o));
-                    acc[r][e] = fma2(acc[r][e], bc2(wa), mul2(other, bc2(wb)));
+                    acc[r][e].x += __shfl_xor_sync(0xffffffffu, acc[r][e].x, o);
+                    acc[r][e].y += __shfl_xor_sync(0xffffffffu, acc[r][e].y, o);
                 }
-            }
-            if (grp == 0) {
+        }
+        if (grp == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) *reinterpret_cast<float2 *>(&s_acc[warp][r][e0 + 2 * e]) = acc[r][e];
-                if (lane == 0) s_ml[warp][r] = make_float2(m[r], l[r]);
-            }
+            if (li % kRowLanes == 0) s_ml[warp][row] = make_float2(m, l);
         }
     }
 };

@@ -44,7 +44,9 @@ __device__ __forceinline__ void halve(float (&s)[N], int lane) {
 template <typename QT, int HD_, int R>
 struct VecCore {
     using Q = QT;
-    static constexpr int HD = HD_, RB = R, kMinBlocks = R <= 4 ? 4 : 2;
+    // of 8 rows, three blocks an SM spill 150 bytes and still pay in long runs (192 us against 225 at the size above, 14 heads on
+    // 2 of 64 55 against 63), but not in small calls (26 against 24 at 8 sequences of 1000 keys)
+    static constexpr int HD = HD_, RB = R, kMinBlocks = R <= 4 ? 4 : 2, kStreamBlocks = R <= 4 ? 4 : 3;
     static constexpr size_t kSmem = 0;
     struct State {};
     static __device__ __forceinline__ void init(State &) {}
@@ -297,13 +299,14 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
     const int64_t resident = !one_tile ? 0
                              : s.mma   ? attn_mma_resident(head_dim, s.rows_blk, dtype)
                                        : with_vec(dtype, head_dim, s.rows_blk, [](auto core) { return rows_resident<decltype(core)>(); });
+    const int64_t fit = s.mma || s.rows_blk < 8 ? resident : std::min(resident, sms * 2);  // clusters' blocks
     if (prefix_len > 0 && one_tile) {
         // one launch of clusters that take the prefix too, by the same rule as below: 8 sequences of up to 1000 rows behind 1003
         // 12.6 us (17.7 in launches apart), 14 heads on 2 of 64 7.9 (14.2)
         int c = 8;
-        while (c > 2 && (base * c > resident || 32 * c > prefix_len + max_kv)) c /= 2;
+        while (c > 2 && (base * c > fit || 32 * c > prefix_len + max_kv)) c /= 2;
         const int64_t cp = std::clamp<int64_t>((c * prefix_len + (prefix_len + max_kv) / 2) / (prefix_len + max_kv), 1, c - 1);
-        if (base * c <= resident && prefix_len <= 512 * cp && max_kv <= 512 * (c - cp)) {
+        if (base * c <= fit && prefix_len <= 512 * cp && max_kv <= 512 * (c - cp)) {
             s.frame = kFrameCluster;
             s.cluster = c, s.cluster_pre = int(cp);
             s.own_units = base;
@@ -332,8 +335,8 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         // with at most 512 keys each, else equal runs of all sequences' tiles: 8 sequences of 1000-2000 keys 12.4 us in clusters
         // (14.1 in runs), 30 of up to 500 5.8 (7.3); one of 8192 keys 13.7 in runs (18.2), of 16384 16.3 (30.6)
         int c = 8;
-        while (c > 1 && (base * c > resident || 32 * c > max_kv)) c /= 2;
-        if (base * c <= resident && max_kv <= 512 * c) {
+        while (c > 1 && (base * c > fit || 32 * c > max_kv)) c /= 2;
+        if (base * c <= fit && max_kv <= 512 * c) {
             s.frame = kFrameCluster;
             s.cluster = c;
             s.own_units = base;

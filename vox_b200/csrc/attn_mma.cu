@@ -3,7 +3,7 @@
 //
 // A warp takes 16 keys a step (32 of 64-wide heads) against 8 or 16 rows. One lane has the tensor copy engine bring K and V
 // tiles of 16 keys x 128 bytes (a page or part of one) into the warp's own ring of two stages in shared memory, so 8 KB a
-// warp (128 KB an SM of four blocks) are in flight at no cost in registers or issue slots; the lanes read 16-byte chunks
+// warp (96 KB an SM of three blocks) are in flight at no cost in registers or issue slots; the lanes read 16-byte chunks
 // back as operands of mma.m16n8k16. Whole chunks serve as operands because the order of a product's summation index is
 // free: S^T = K Q^T sums over the head's elements, so lane (g, t) may supply of key g the 16-byte chunks t, t + 4, .. as they
 // lie in memory, if Q's operand takes the same chunks; and O^T = V^T P^T has V's elements as its rows, so lane (g, t) loads
@@ -58,7 +58,8 @@ template <typename QT, int HD_, int NT>
 struct MmaCore {
     using Q = QT;
     static constexpr int HD = HD_, RB = 8 * NT;
-    static constexpr int kMinBlocks = NT == 2 || sizeof(QT) == 4 ? 2 : 3;
+    static constexpr int kStreamBlocks = NT == 2 || sizeof(QT) == 4 ? 2 : 3;
+    static constexpr int kMinBlocks = kStreamBlocks;
     static constexpr int kStages = 2;
     static constexpr uint32_t kBox = 16 * 128;    // bytes of a box: 16 keys x 64 elements
     static constexpr uint32_t kStage = 4 * kBox;  // K and V of a step: 2 halves of 16 keys, or 32 keys of 64-wide heads

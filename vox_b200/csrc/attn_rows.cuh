@@ -1,7 +1,7 @@
 // The frame around the kernels of few query rows (attn.cu on f32 caches, attn_mma.cu on bf16 caches): which rows and keys a
 // block takes, and where its result goes. A core computes softmax statistics and unnormalised output of up to RB rows over
 // a range of keys, one part a warp, into shared memory:
-//   struct Core { static constexpr int HD, RB, kMinBlocks; static constexpr size_t kSmem (dynamic shared memory); using Q = ...;
+//   struct Core { static constexpr int HD, RB, kMinBlocks, kStreamBlocks (blocks an SM, of the stream frame); static constexpr size_t kSmem (dynamic shared memory); using Q = ...;
 //                 struct State (of a thread, through all its jobs); static void init(State &); static (*acc(State &))[RB][HD];
 //                 static void run(const AttnArgs &, const RowsJob &, float (*acc)[RB][HD], float2 (*ml)[RB], State &, F between); };
 // (between() is called by every thread while the first copies of the job are on their way.)
@@ -277,7 +277,7 @@ __device__ __forceinline__ void stream_next(const AttnArgs &a, StreamState &st, 
 }
 
 template <class Core>
-__global__ void __launch_bounds__(kRowsThreads, Core::kMinBlocks) attn_stream_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, Core::kStreamBlocks) attn_stream_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int HD = Core::HD, RB = Core::RB;
     __shared__ float2 s_ml[kRowsWarps][RB];
     __shared__ int s_part[kRowsWarps];

@@ -354,8 +354,9 @@ VOX_CUDA_API int vox_cuda_attn_paged(const vox_cuda_kv_cache *cache, const vox_c
 
 /* The same attention for a batch whose sequences all stand behind one shared prefix (a voice prompt): every token sees the
  * prefix_len rows behind prefix_pages (device, ceil(prefix_len / page_size) page numbers), then its own sequence's rows as
- * above (kv_len counts the sequence's own rows). The prefix is read once for the whole batch, not once a sequence; the two
- * parts' softmax statistics are joined exactly. prefix_len 0 is vox_cuda_attn_paged. */
+ * above (kv_len counts the sequence's own rows). The prefix is read for the rows of the whole batch together, unless the call
+ * is so small, or its texts so long, that a walk of its own costs more than reading it for every sequence; the two parts'
+ * softmax statistics are joined exactly. prefix_len 0 is vox_cuda_attn_paged. */
 VOX_CUDA_API int vox_cuda_attn_prefix(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, const int32_t *prefix_pages,
                                       int64_t prefix_len, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                                       int64_t heads, float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);

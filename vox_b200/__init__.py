@@ -646,7 +646,7 @@ class PagedKV:
     def attend_prefix(self, q, prefix_pages, prefix_len: int, page_table, kv_len, q_start=None, max_q: int = 0, max_kv: int = 0,
                       scale: float | None = None, out=None) -> torch.Tensor:
         """attend() for sequences that all stand behind one shared prefix: every token sees the prefix_len rows behind
-        prefix_pages (int32), read once for the whole batch, and then its own sequence's rows as in attend()."""
+        prefix_pages (int32), read for the whole batch together, and then its own sequence's rows as in attend()."""
         if not (isinstance(prefix_pages, torch.Tensor) and prefix_pages.dtype is torch.int32 and prefix_pages.get_device() == self._dev and
                 prefix_pages.dim() == 1 and prefix_pages.is_contiguous()):
             raise VoxCudaError(-6, "prefix_pages must be a contiguous int32 tensor on the cache's device")

@@ -595,6 +595,29 @@ def test_rows_where_the_kernels_change(vox, act, cache, q, prefix):
     assert vox.device_error() == 0
 
 
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("hd,prefix", [(64, 0), (128, 0), (128, 333), (64, 70)])
+def test_many_short_prompts(vox, page, hd, prefix):
+    """Prompts of at most 128 rows, more of them than the device has room for at once: with and without cached rows in front,
+    ends before, at and past steps of 64 keys, a window, sequences longer than max_q and max_kv say."""
+    r = np.random.default_rng(page)
+    lens = [(int(n), int(n) + int(e)) for n, e in zip(r.integers(1, 65, 30), r.integers(0, 300, 30))]
+    lens[:6] = [(64, 64), (63, 65), (64, 128), (1, 129), (0, 70), (64, 513)]
+    bt = Batch(lens, 8, hd, page, BF16, seed=page, prefix=prefix)
+    q = queries(bt, 16, BF16)
+    table, kv_len, q_start = bt.dev()
+    h, pre = bt.handle(vox), bt.prefix_pages.cuda()
+    want, mag, big = attention64(bt, q, 16, hd ** -0.5)
+    for mq, mkv in ((64, 513), (20, 100), (40, 0)):
+        kw = dict(q_start=q_start, max_q=mq, max_kv=mkv)
+        got = h.attend_prefix(q.cuda(), pre, prefix, table, kv_len, **kw) if prefix else h.attend(q.cuda(), table, kv_len, **kw)
+        check(got, want, mag, big, BF16, BF16, 900)
+    if not prefix:
+        want, mag, big = attention64(bt, q, 16, hd ** -0.5, window=90)
+        check(h.attend(q.cuda(), table, kv_len, q_start=q_start, max_q=64, window=90), want, mag, big, BF16, BF16, 900)
+    assert vox.device_error() == 0
+
+
 @pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
 def test_scores_that_keep_rising(vox, act, cache):
     """Every step's largest score is far above the last one's, so the running maximum moves at each; and far below, so it

@@ -252,6 +252,7 @@ struct AttnShape {
     bool wide, pre_wide;               // or, many rows at f32 accuracy, to attn_f32.cu (the prefix alone, in a launch of its own)
     int frame;                         // of the own keys, where the tensor-core kernel does not take them
     int rows_blk, tc_rows;
+    bool tc_half;                      // blocks of one row tile of the tensor-core kernel
     int own_tiles, own_splits, own_chunk;
     int pre_tiles, pre_splits, pre_chunk;
     int cluster, cluster_pre, stream_shift, stream_rows;
@@ -288,6 +289,11 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
     // row tiles of all sequences together: no more than `bound` (the launch covers it), and `tiles` where max_q holds
     auto bound = [&](int64_t rb) { return p.q_start ? (all - p.seqs) / rb + p.seqs : p.seqs * ((rows + rb - 1) / rb); };
     auto tiles = [&](int64_t rb) { return std::max<int64_t>(std::min(bound(rb), p.seqs * ((rows + rb - 1) / rb)), 1); };
+    // Blocks of one row tile, two an SM, where no sequence has more and there are more than one an SM: a block's start and end
+    // lie behind the other's walk: 24 texts of 128 rows behind 1003 28.8 us (37.8 in blocks of two tiles), of 64 29.2 (36.3), 64 prompts
+    // of 120 rows 28.9 (41.3). With fewer blocks their stages of half the size cost more: 64 rows on each of 16 sequences of 2000
+    // keys 49 against 35; and so do long rows (8192 tokens 271 against 234: every tile of keys is read for half as many rows)
+    s.tc_half = s.own_tc && rows <= 128 && tiles(128) * p.kv_heads > sms;
     // The prefix in front of each text's own keys in the same block, without a join; or apart, for the rows of all texts
     // together, which fill their row tiles: apart if that spares an SM more than ten tiles of 128 keys, or the texts are short.
     // 24 texts behind 1003 rows: 128 rows a text 37.2 us (38.9 apart), 200 rows 54.9 (57.9), 14-300 rows 52 (50.7), 64 rows 36.2
@@ -314,7 +320,7 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         }
     }
     if (prefix_len > 0 && !s.concat) {
-        const int rb = s.pre_tc ? (all > 128 ? 256 : 128) : s.pre_wide ? kF32Rows : s.rows_blk;
+        const int rb = s.pre_tc ? (all > 128 && !s.tc_half ? 256 : 128) : s.pre_wide ? kF32Rows : s.rows_blk;
         if (s.pre_tc) s.tc_rows = rb;
         s.pre_tiles = ceil_div(all, rb);
         const int64_t pre = int64_t(p.kv_heads) * s.pre_tiles;
@@ -325,7 +331,7 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
         // both row tiles of a block on different rows halve the reads of keys and fill its softmax's gaps, but halve the blocks:
         // one prompt of 300 tokens 12.6 us with 128 rows a block (14.4 with 256), of 1000 20.2 (23.0); 24 texts of 7-150 tokens
         // behind 1003 rows 52 with 256 (63)
-        if (s.tc_rows == 0) s.tc_rows = tiles(256) * p.kv_heads >= sms / 2 ? 256 : 128;
+        if (s.tc_rows == 0) s.tc_rows = !s.tc_half && tiles(256) * p.kv_heads >= sms / 2 ? 256 : 128;
         s.own_tiles = int(bound(s.tc_rows));
         const int64_t busy = tiles(s.tc_rows) * p.kv_heads;
         cut_keys(max_kv, s.concat ? 1 : busy < sms ? sms / busy : 1, s.own_splits, s.own_chunk);
@@ -427,7 +433,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.splits = s.slots, a.partial = w.partial;
     a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
     a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;
-    a.tc_rows = s.tc_rows, a.concat = s.concat;
+    a.tc_rows = s.tc_rows, a.tc_half = s.tc_half, a.concat = s.concat;
     a.cluster = s.cluster, a.cluster_pre = s.cluster_pre, a.stream_shift = s.stream_shift, a.stream_rows = s.stream_rows, a.stream_rb = s.rows_blk;
     a.stream_blocks = int32_t(s.frame == kFrameStream ? s.own_units : 0);
     char *scratch = static_cast<char *>(workspace);

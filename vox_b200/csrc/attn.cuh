@@ -30,14 +30,14 @@ struct AttnArgs {
     FastDiv kvdiv, otdiv, osdiv, ptdiv, srdiv; // divisions by kv_heads, seqs * own_splits, own_splits, pre_tiles, stream_rows
     int32_t pre_blocks, splits;                // blocks of the prefix (they come first); slots of a row in the workspace
     int32_t partial;                           // results go to the workspace (a row's parts meet in a later launch)
-    // the tensor-core kernel: rows a block; whether this launch takes the prefix; whether the own keys follow the prefix
-    // in one walk (then pre_splits is 0). own_tiles counts the row tiles of all sequences there.
-    int32_t tc_rows, concat;
+    // the tensor-core kernel: rows a block; whether its blocks have one row tile, two of them an SM; whether the own keys
+    // follow the prefix in one walk (then pre_splits is 0). own_tiles counts the row tiles of all sequences there.
+    int32_t tc_rows, tc_half, concat;
     // there the scale is positive (row maxima are taken before it): a negative one flips q's signs, zero clears q
     float tc_scale;
     uint32_t q_and, q_xor;
-    // few query rows (attn_rows.cuh): blocks a cluster and how many of them take the prefix; or log2 of the keys a tile of the list, rows that the joining launch looks at,
-    // rows and number of the parts, and the parts themselves
+    // few query rows (attn_rows.cuh): blocks a cluster and how many of them take the prefix; or log2 of the keys a tile of
+    // the list, rows that the joining launch looks at, rows and number of the parts, and the parts themselves
     int32_t cluster, cluster_pre, stream_shift, stream_rows, stream_rb, stream_blocks;
     float *stream_o;
     float2 *stream_ml;

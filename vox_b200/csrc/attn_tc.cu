@@ -13,6 +13,8 @@
 //                   page); rows of V past the last key are zeroed (their weight is 0, and 0 times what lies there may be NaN)
 //   warps 9, 10     issue the products of row tile 0, 1: P V of a step, then Q K^T two steps on into the same S buffer
 // Tile order in the ring: K0 V0 K1 V1 ... (both row tiles read each). Every wait is bounded.
+// QT 1: the same with one row tile, stages of 64 keys and half of the tensor memory, so that two blocks share an SM (many
+// short texts; the rule is in attn.cu). Below, roles and columns are QT 2's.
 //
 // Measured: one prompt of 8192 tokens, 16 query heads on 8 of 128, 231 us in a graph: 1190 TFLOP/s of the causal half, 0.71 of
 // what a bare product reaches. Bound by the softmax, some 1610 clocks per 64 keys of both row tiles (exponentials, their
@@ -22,6 +24,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "attn.cuh"
@@ -31,9 +34,9 @@
 namespace voxcuda {
 namespace {
 
-constexpr int kKeys = 128;  // keys a stage; a softmax step takes half of them
 constexpr int kStepKeys = 64;
-constexpr int kTcThreads = 352;
+constexpr int tc_keys(int qt) { return 64 * qt; }  // keys a stage
+constexpr int tc_threads(int qt) { return 32 * (5 * qt + 1); }
 constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 
 // Which of eight pairs of weights take ex2_poly. 1, 2, 3 or 4 of them: 230.6, 231.3, 238, 247 us at one prompt of 8192 tokens
@@ -41,24 +44,26 @@ constexpr uint32_t kHalf = 128 * 128;  // bytes of 128 rows of 64 bf16
 constexpr int POLY = 0x11;
 
 constexpr int tc_stages(int hd) { return hd == 128 ? 4 : 8; }
-constexpr size_t tc_smem(int hd) { return 1024 + size_t(2 + tc_stages(hd)) * (hd / 64) * kHalf + 512; }
+constexpr size_t tc_smem(int hd, int qt) { return 1024 + size_t(qt) * (hd / 64) * (kHalf + size_t(tc_stages(hd)) * (kHalf / 2)) + 512; }
 
 // The products of one tile, issued by one elected lane of a converged warp in one piece of code (the issuing warp runs once
 // a tile between long stretches of softmax code, so its instructions are cold: few of them matter).
-// S = Q K^T: HD / 16 steps; both operands K-major, 32 bytes a step, the second 64 elements kHalf bytes on.
-template <int HD>
+// S = Q K^T: HD / 16 steps; both operands K-major, 32 bytes a step, the second 64 elements of Q kHalf bytes on, of K KS 128.
+template <int HD, int KS>
 __device__ __forceinline__ void umma_qk_warp(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint64_t *bar) {
-#define VOX_QK_STEP(OFF, P) "add.s64 a, %1, " OFF ";\n\tadd.s64 b, %2, " OFF ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, " P ";\n\t"
+#define VOX_QK_STEP(QOFF, KOFF, P) "add.s64 a, %1, " QOFF ";\n\tadd.s64 b, %2, " KOFF ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, " P ";\n\t"
 #define VOX_QK_HEAD "{\n\t.reg .pred e, z, o;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 z, 0, 0;\n\tsetp.eq.b32 o, 0, 0;\n\t"
 #define VOX_COMMIT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}"
     if constexpr (HD == 128)
-        asm volatile(VOX_QK_HEAD VOX_QK_STEP("0", "z") VOX_QK_STEP("2", "o") VOX_QK_STEP("4", "o") VOX_QK_STEP("6", "o") VOX_QK_STEP("1024", "o")
-                         VOX_QK_STEP("1026", "o") VOX_QK_STEP("1028", "o") VOX_QK_STEP("1030", "o") VOX_COMMIT ::"r"(d),
-                     "l"(da), "l"(db), "r"(idesc), "r"(smem_addr(bar))
+        asm volatile(VOX_QK_HEAD VOX_QK_STEP("0", "0", "z") VOX_QK_STEP("2", "2", "o") VOX_QK_STEP("4", "4", "o") VOX_QK_STEP("6", "6", "o")
+                         VOX_QK_STEP("1024", "%5", "o") VOX_QK_STEP("1026", "%5+2", "o") VOX_QK_STEP("1028", "%5+4", "o")
+                             VOX_QK_STEP("1030", "%5+6", "o") VOX_COMMIT ::"r"(d),
+                     "l"(da), "l"(db), "r"(idesc), "r"(smem_addr(bar)), "n"(KS * 8)
                      : "memory");
     else
-        asm volatile(VOX_QK_HEAD VOX_QK_STEP("0", "z") VOX_QK_STEP("2", "o") VOX_QK_STEP("4", "o") VOX_QK_STEP("6", "o") VOX_COMMIT ::"r"(d), "l"(da),
-                     "l"(db), "r"(idesc), "r"(smem_addr(bar))
+        asm volatile(VOX_QK_HEAD VOX_QK_STEP("0", "0", "z") VOX_QK_STEP("2", "2", "o") VOX_QK_STEP("4", "4", "o") VOX_QK_STEP("6", "6", "o")
+                         VOX_COMMIT ::"r"(d),
+                     "l"(da), "l"(db), "r"(idesc), "r"(smem_addr(bar))
                      : "memory");
 }
 // O (+)= P V over 64 keys, 16 a step: P in TMEM (two bf16 a column: 8 columns a step), V MN-major (2048 bytes a step); acc:
@@ -170,62 +175,62 @@ __device__ __forceinline__ void tc_job(const AttnArgs &a, uint32_t blk, TcJob &o
     if (lane == 0) out = j;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kTcThreads, 1)
+template <int HD, int QT>
+__global__ void __launch_bounds__(tc_threads(QT), QT == 1 ? 2 : 1)
     attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
-    constexpr int NS = tc_stages(HD), H = HD / 64;
-    constexpr uint32_t kTile = H * kHalf;
+    constexpr int NS = tc_stages(HD), H = HD / 64, KS = tc_keys(QT), SPS = KS / kStepKeys;  // SPS: steps a stage
+    constexpr int kCopyWarp = 4 * QT, kMmaWarp = kCopyWarp + 1;
+    constexpr uint32_t kTile = H * kHalf, kSub = KS * 128, kStage = H * kSub;  // bytes: a Q tile; 64 columns of a stage; a stage
     constexpr uint32_t kIdS = umma_idesc_bf16(128, kStepKeys), kIdO = umma_idesc_bf16(128, HD, true);
     extern __shared__ uint8_t raw[];
     __shared__ TcJob job;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t sQ = smem_addr(smem), sKV = sQ + 2 * kTile;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + (2 + NS) * kTile), *empty = full + NS;
+    const uint32_t sQ = smem_addr(smem), sKV = sQ + QT * kTile;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + QT * kTile + NS * kStage), *empty = full + NS;
     uint64_t *s_full = empty + NS, *p_full = s_full + 4, *o_done = p_full + 4, *o_full = o_done + 2, *q_full = o_full + 2, *tail = q_full + 2, *drain = tail + 1;
     uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_enter();
     if (warp == 0) tc_job(a, blockIdx.x, job);
     if (threadIdx.x == 32) {
-        for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 2);
+        for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], QT);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
         for (int q = 0; q < 2; ++q) mbar_init(&q_full[q], 4), mbar_init(&o_done[q], 1), mbar_init(&o_full[q], 1);
         mbar_init(tail, 1);
-        mbar_init(drain, 2);
+        mbar_init(drain, QT);
         mbar_init_fence();
     }
-    if (warp == 9) tmem_alloc(tslot, 512);
+    if (warp == kMmaWarp) tmem_alloc(tslot, 256 * QT);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const TcJob j = job;
     const uint32_t tmem = *tslot;
     if (!j.ok) {
-        if (warp == 9) tmem_dealloc(tmem, 512);
+        if (warp == kMmaWarp) tmem_dealloc(tmem, 256 * QT);
         return;
     }
-    // key tiles of 128: nA of the prefix, then the own keys from kb0; hi of a row tile = keys that its last row sees; nt = its
+    // key tiles of a stage: nA of the prefix, then the own keys from kb0; hi of a row tile = keys that its last row sees; nt = its
     // steps of 64 keys
-    const int nA = (j.pa1 - j.pa0 + kKeys - 1) / kKeys;
+    const int nA = (j.pa1 - j.pa0 + KS - 1) / KS;
     int kb0 = j.k0;
     if (a.window > 0 && j.causal) {
         const int first = int(a.gdiv.div(uint32_t(j.row0)));
-        kb0 = max(kb0, max(j.base + first + 1 - a.window, 0) & ~(kKeys - 1));
+        kb0 = max(kb0, max(j.base + first + 1 - a.window, 0) & ~(KS - 1));
     }
-    int nt[2], kend = 0;
+    int nt[2] = {0, 0}, kend = 0;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < QT; ++q) {
         const int r0 = j.row0 + 128 * q;
-        nt[q] = 0;
         if (r0 < j.rows && 128 * q < a.tc_rows) {
             const int last = int(a.gdiv.div(uint32_t(min(r0 + 127, j.rows - 1))));
             const int hi = j.causal ? min(j.base + last + 1, j.k1) : 0;
-            nt[q] = 2 * nA + max(hi - kb0 + kStepKeys - 1, 0) / kStepKeys;
+            nt[q] = SPS * nA + max(hi - kb0 + kStepKeys - 1, 0) / kStepKeys;
             kend = max(kend, hi);
         }
     }
-    const int nmax = (max(nt[0], nt[1]) + 1) / 2;  // tiles of 128
-    if (warp < 8) {
+    const int nmax = (max(nt[0], nt[1]) + SPS - 1) / SPS;
+    if (warp < kCopyWarp) {
         // ---------------------------------------------------------------- softmax: thread = row
         {   // the row tile's Q: 16-byte chunks of whole rows, every load in flight before the first is stored, 128-byte
             // swizzle; rows past the end are zero
@@ -256,7 +261,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         const int q = warp >> 2, row = (warp & 3) * 32 + lane, rr = j.row0 + 128 * q + row;
         const int n = q ? nt[1] : nt[0];
-        const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16), tO = lanes + 256 + HD * q;
+        const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16), tO = lanes + 128 * QT + HD * q;
         const bool live = rr < j.rows && 128 * q < a.tc_rows;
         const int i_tok = int(a.gdiv.div(uint32_t(live ? rr : 0)));
         const int hi_own = live && j.causal ? min(j.base + i_tok + 1, j.k1) : 0;
@@ -275,8 +280,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
             tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r));
             tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r + 32));
-            const bool pre = u < 2 * nA;
-            const int key0 = pre ? j.pa0 + u * kStepKeys : kb0 + (u - 2 * nA) * kStepKeys;
+            const bool pre = u < SPS * nA;
+            const int key0 = pre ? j.pa0 + u * kStepKeys : kb0 + (u - SPS * nA) * kStepKeys;
             const int hi = (pre ? (live ? j.pa1 : 0) : hi_own) - key0, lo = (pre ? j.pa0 : lo_own) - key0;
             if (!__all_sync(0xffffffffu, hi >= kStepKeys && lo <= 0)) {
 #pragma unroll
@@ -401,35 +406,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
         }
         if (live && ok && a.partial) a.part_ml[slot] = make_float2(ref, l);
-    } else if (warp == 8) {
+    } else if (warp == kCopyWarp) {
         // ---------------------------------------------------------------- copies
-        const int pr = min(a.p.page_mask + 1, kKeys);  // rows a box
+        const int pr = min(a.p.page_mask + 1, KS);  // rows a box
         bool ok = true;
         int tails = 0, n = 0;
         for (; n < 2 * nmax && ok; ++n) {
             const int i = n >> 1, s = n % NS;
             const bool is_v = n & 1, pre = i < nA;
-            const int key0 = pre ? j.pa0 + i * kKeys : kb0 + (i - nA) * kKeys;
-            const int valid = min((pre ? j.pa1 : kend) - key0, kKeys);
+            const int key0 = pre ? j.pa0 + i * KS : kb0 + (i - nA) * KS;
+            const int valid = min((pre ? j.pa1 : kend) - key0, KS);
             if (n >= NS) ok = wait_soon(&empty[s], uint32_t(n / NS - 1) & 1u);
             if (!ok) break;
             const int boxes = (valid + pr - 1) / pr * H;
-            const bool zero = is_v && valid < kKeys;
+            const bool zero = is_v && valid < KS;
             uint64_t *bar = zero ? tail : &full[s];
-            const uint32_t st = sKV + s * kTile;
+            const uint32_t st = sKV + s * kStage;
             if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(boxes * pr) * 128u);
             __syncwarp();
             if (lane < boxes) {
                 const int p = lane / H, half = lane % H, key = key0 + p * pr;
                 const int page = page_checked(a.p, __ldg((pre ? a.prefix_pages : j.pages) + (key >> a.p.page_shift)));
-                tma_load_4d(st + half * kHalf + p * pr * 128, is_v ? &mv : &mk, half * 64, j.kvh, key & a.p.page_mask, page, bar);
+                tma_load_4d(st + half * kSub + p * pr * 128, is_v ? &mv : &mk, half * 64, j.kvh, key & a.p.page_mask, page, bar);
             }
             if (zero) {
                 ok = wait_soon(tail, uint32_t(tails++ & 1));
-                for (int x = valid * 8 + lane; x < kKeys * 8; x += 32)
+                for (int x = valid * 8 + lane; x < KS * 8; x += 32)
 #pragma unroll
                     for (int half = 0; half < H; ++half)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(st + half * kHalf + x * 16), "r"(0) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(st + half * kSub + x * 16), "r"(0) : "memory");
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[s]);
@@ -439,19 +444,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int m = max(n - NS, 0); m < n; ++m) wait_soon(&full[m % NS], uint32_t(m / NS) & 1u);
     } else {
         // ---------------------------------------------------------------- products of row tile q
-        const int q = warp - 9, n = q ? nt[1] : nt[0];
+        const int q = warp - kMmaWarp, n = q ? nt[1] : nt[0];
         bool ok = true;
         auto wait_full = [&](int m) { return wait_soon(&full[m % NS], uint32_t(m / NS) & 1u); };
-        constexpr uint32_t kStep = kTile >> 4, kSub = kStepKeys * 128 >> 4;  // a tile, half a tile's rows on, in descriptor units
-        const uint64_t dQ = umma_desc(sQ + q * kTile, 16, 1024), dK = umma_desc(sKV, 16, 1024), dV = umma_desc(sKV, kHalf, 1024);
-        const uint32_t tS = tmem + 128 * q, tO = tmem + 256 + HD * q;
+        constexpr uint32_t kNext = kStage >> 4, kHalfStage = kStepKeys * 128 >> 4;  // a stage, a step's keys on, in descriptor units
+        const uint64_t dQ = umma_desc(sQ + q * kTile, 16, 1024), dK = umma_desc(sKV, 16, 1024), dV = umma_desc(sKV, kSub, 1024);
+        const uint32_t tS = tmem + 128 * q, tO = tmem + 128 * QT + HD * q;
         auto qk = [&](int u) {  // scores of step u; the last step of a tile gives K back
-            const int m = u & ~1;
-            if (!(u & 1)) ok = wait_full(m);
+            const int m = u / SPS * 2, sub = u % SPS;
+            if (sub == 0) ok = wait_full(m);
             if (!ok) return;
             tc_fence_after();
-            umma_qk_warp<HD>(tS + 64 * (u & 1), dQ, dK + uint32_t(m % NS) * kStep + (u & 1) * kSub, kIdS, &s_full[2 * q + (u & 1)]);
-            if ((u & 1) || u + 1 == n) umma_commit_warp(&empty[m % NS]);
+            umma_qk_warp<HD, KS>(tS + 64 * (u & 1), dQ, dK + uint32_t(m % NS) * kNext + sub * kHalfStage, kIdS, &s_full[2 * q + (u & 1)]);
+            if (sub == SPS - 1 || u + 1 == n) umma_commit_warp(&empty[m % NS]);
         };
         if (n > 0) {
             ok = wait_soon(&q_full[q], 0);
@@ -460,18 +465,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
 #pragma unroll 1
         for (int u = 0; u < n && ok; ++u) {
-            const int m = u | 1;  // V of the tile
-            if (!(u & 1)) ok = wait_full(m);
+            const int m = u / SPS * 2 + 1, sub = u % SPS;  // V of the stage
+            if (sub == 0) ok = wait_full(m);
             ok = ok && wait_soon(&p_full[2 * q + (u & 1)], uint32_t(u >> 1) & 1u);
             if (!ok) break;
             tc_fence_after();
-            umma_pv_warp(tO, tS + 64 * (u & 1), dV + uint32_t(m % NS) * kStep + (u & 1) * kSub, kIdO, uint32_t(u > 0), &o_done[q]);
-            if ((u & 1) || u + 1 == n) umma_commit_warp(&empty[m % NS]);
+            umma_pv_warp(tO, tS + 64 * (u & 1), dV + uint32_t(m % NS) * kNext + sub * kHalfStage, kIdO, uint32_t(u > 0), &o_done[q]);
+            if (sub == SPS - 1 || u + 1 == n) umma_commit_warp(&empty[m % NS]);
             if (u + 1 == n) umma_commit_warp(&o_full[q]);
             if (u + 2 < n) qk(u + 2);
         }
         // tiles that only the other row tile reads: given back as they come (a stage is free when both warps have said so)
-        for (int m = (n + 1) / 2 * 2; m < 2 * nmax && ok; ++m) {
+        for (int m = (n + SPS - 1) / SPS * 2; m < 2 * nmax && ok; ++m) {
             ok = wait_full(m);
             if (ok && lane == 0) mbar_arrive(&empty[m % NS]);
         }
@@ -481,9 +486,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, 256 * QT);
     }
 }
 
@@ -501,11 +506,11 @@ PFN_cuTensorMapEncodeTiled_v12000 encode() {
     return fn;
 }
 
-template <int HD>
+template <int HD, int QT>
 int launch(const AttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int64_t blocks, cudaStream_t st, const char *name) {
-    auto kern = attn_tc_kernel<HD>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tc_smem(HD))) != cudaSuccess) return check_launch(name);
-    launch_k(kern, dim3(unsigned(blocks)), kTcThreads, tc_smem(HD), st, a, mk, mv);
+    auto kern = attn_tc_kernel<HD, QT>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tc_smem(HD, QT))) != cudaSuccess) return check_launch(name);
+    launch_k(kern, dim3(unsigned(blocks)), tc_threads(QT), tc_smem(HD, QT), st, a, mk, mv);
     return check_launch(name);
 }
 
@@ -528,11 +533,12 @@ int attn_cache_map(const vox_cuda_kv_cache &c, const void *base, int box_rows, C
 
 int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks, cudaStream_t st, const char *name) {
     CUtensorMap mk, mv;
-    const int rows = c.page_size < kKeys ? c.page_size : kKeys;  // a box never leaves a page
+    const int qt = a.tc_half ? 1 : 2, rows = std::min(c.page_size, tc_keys(qt));  // a box never leaves a page
     int rc = attn_cache_map(c, c.k, rows, mk, name);
     if (rc == VOX_CUDA_OK) rc = attn_cache_map(c, c.v, rows, mv, name);
     if (rc != VOX_CUDA_OK) return rc;
-    return c.head_dim == 64 ? launch<64>(a, mk, mv, blocks, st, name) : launch<128>(a, mk, mv, blocks, st, name);
+    if (c.head_dim == 64) return qt == 1 ? launch<64, 1>(a, mk, mv, blocks, st, name) : launch<64, 2>(a, mk, mv, blocks, st, name);
+    return qt == 1 ? launch<128, 1>(a, mk, mv, blocks, st, name) : launch<128, 2>(a, mk, mv, blocks, st, name);
 }
 
 int attn_tc_take_device_error(unsigned int *flags) { return take_device_error(flags); }

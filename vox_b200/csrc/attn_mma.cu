@@ -17,7 +17,7 @@
 //
 // Measured (one token a sequence, 16 query heads on 8 of 128): 16 sequences of 20-32 k keys 238 us, 6.7 TB/s, the rate of a
 // plain copy. Shorter calls pay the start of the loads (length scan, page look-up, first copies: some 5 us) and the join (see
-// attn_rows.cuh): 96 ragged streams of 14 heads on 2 of 64 take 34.5 us, 33 of 16 on 8 of 128 with f32 activations 41. With
+// attn_rows.cuh): 96 ragged streams of 14 heads on 2 of 64 take 32.5 us, 33 of 16 on 8 of 128 with f32 activations 41. With
 // the chunks loaded from memory into registers instead of copied to a ring, f32 activations 49 us and long bf16 streams
 // 250; with three stages, and so fewer blocks an SM, 62 against 46 at the same step.
 #include "attn_rows.cuh"

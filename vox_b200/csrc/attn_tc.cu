@@ -525,8 +525,11 @@ int attn_cache_map(const vox_cuda_kv_cache &c, const void *base, int box_rows, C
     const cuuint64_t strides[3] = {cuuint64_t(head) * 2, cuuint64_t(c.row_stride) * 2, cuuint64_t(page) * 2};
     const cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
     const cuuint32_t es[4] = {1, 1, 1, 1};
+    // L2 fetches a head's row at a time: with 256 bytes a 64-wide head's neighbour comes too and some of it is fetched again (96
+    // ragged streams of 14 heads on 2: 33.8 us and 161 MB against 32.2 at 146 MB of rows)
+    const CUtensorMapL2promotion promotion = c.head_dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
     const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(VOX_CUDA_ERR_ARG, std::string(name) + ": cache tensor map rejected (code " + std::to_string(int(r)) + ")");
     return VOX_CUDA_OK;
 }

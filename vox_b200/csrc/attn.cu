@@ -36,11 +36,13 @@ __device__ __forceinline__ void halve(float (&s)[N], int lane) {
 // bytes, so a warp load brings KPW keys (one a group of LPK lanes); a step takes U of them. The U R dot products of a step are
 // summed over the group by halving: a lane gives half of its values away at each exchange and adds what it gets to the
 // other half, so it ends with the whole sum of one (row, key) pair (or C of them, or D lanes with the same one), takes its
-// 2^x alone, keeps the sum of its weights, and hands the weights to the group through shared memory. That is about one exchange a
-// score. (A butterfly for each, every lane taking every 2^x: 201 us against 139 at 32 sequences of 2000-4000 keys and 4 rows, 369
-// against 227 at 8.) The rows' references are the warp's
-// and move only when a score exceeds one by 8 (base 2): the common step has one vote. Every warp takes each kRowsWarps-th
-// run of KPI keys; from four rows on, the next step's K is loaded while this one's weights and products are worked on.
+// 2^x alone, keeps the sum of its weights, and hands the weights to the group through shared memory. That is about one
+// exchange a score. (A butterfly for each, every lane taking every 2^x: 201 us against 139 at 32 sequences of 2000-4000 keys
+// and 4 rows, 369 against 227 at 8.) The rows' references are the warp's and move only when a score exceeds one by 8 (base 2):
+// the common step has one vote. Every warp takes each kRowsWarps-th run of KPI keys; from four rows on, the next step's K is
+// loaded while this one's weights and products are worked on (without it 169 us for 139, 297 for 225).
+// At that size, 8 heads of 128: 2 rows 130 us (6.3 TB/s), 4 rows 139, 8 rows 192 (bound by the exchanges and additions). One token
+// over 650 keys takes 8.4 us in a graph: latency (its 5 MB would need 0.8).
 template <typename QT, int HD_, int R>
 struct VecCore {
     using Q = QT;
@@ -429,7 +431,8 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     a.own_splits = s.own_splits, a.own_chunk = s.own_chunk, a.own_tiles = s.own_tiles;
     a.pre_splits = s.pre_splits, a.pre_chunk = s.pre_chunk, a.pre_tiles = s.pre_tiles;
     auto div_by = [](int d) { return FastDiv(uint32_t(d > 0 ? d : 1)); };
-    a.kvdiv = div_by(a.p.kv_heads), a.otdiv = div_by(a.p.seqs * (s.own_splits > 0 ? s.own_splits : 1)), a.osdiv = div_by(s.own_splits), a.ptdiv = div_by(s.pre_tiles), a.srdiv = div_by(s.stream_rows);
+    a.kvdiv = div_by(a.p.kv_heads), a.otdiv = div_by(a.p.seqs * (s.own_splits > 0 ? s.own_splits : 1)), a.osdiv = div_by(s.own_splits);
+    a.ptdiv = div_by(s.pre_tiles), a.srdiv = div_by(s.stream_rows);
     a.splits = s.slots, a.partial = w.partial;
     a.tc_scale = scale == 0.f ? 1.f : fabsf(a.scale_log2);
     a.q_and = scale == 0.f ? 0u : ~0u, a.q_xor = scale < 0.f ? 0x80008000u : 0u;

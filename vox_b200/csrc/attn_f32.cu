@@ -1,8 +1,8 @@
 // The paged attention of many query rows where f32 accuracy is asked for (f32 activations, or an f32 cache): prompts of the
 // CPU engine's own precision. Flash attention on the tensor cores in TF32 with operands cut in two, which keeps f32 accuracy:
-// x = hi + lo of 11 significant bits each, and x y = hi hi + hi lo + lo hi up to 2^-21 (a bf16 key or
-// value has no lo part: two products). A block takes 64 rows (16 a warp) of one key/value head, the heads that share it side
-// by side, and walks the keys in tiles of 32 that its four warps share in shared memory (asynchronous copies, two buffers).
+// x = hi + lo of 11 significant bits each, and x y = hi hi + hi lo + lo hi up to 2^-21 (a bf16 key or value has no lo part:
+// two products). A block takes 64 rows (16 a warp) of one key/value head, the heads that share it side by side, and walks the
+// keys in tiles of 32 that its four warps share in shared memory (asynchronous copies, two buffers).
 //   S = Q K^T, m16n8k8: the summation index may run in any order, so a lane takes 16-byte chunks of Q's and K's rows as they
 //   lie and uses their words two by two; P's accumulator layout (a row, keys 2t and 2t + 1) is the next product's operand
 //   layout if V's rows are taken in that order, and V's chunks of four elements serve four column tiles, so nothing is
@@ -13,8 +13,8 @@
 // truncation at the size of the hi sum would swallow, have sums of their own: largest error against 64 bits 5.0e-7 of the
 // output's scale, as against 1.1e-6 in one sum (sums in f32 by plain matrix products: 6.3e-7).
 // Bound by the issue and latency of the products (three mma of 16 x 8 x 8 a step, and the cutting of operands between), not by
-// bytes: 5 ragged prompts of 90-700 tokens, 16 heads of 64, take 113 us where their bytes would need 6. Two blocks an SM
-// (at most 255 registers, nothing spilled) 113 us against 125 with one and 117 with operands that spill.
+// bytes: 5 ragged prompts of 90-700 tokens, 16 heads of 64, take 113 us where their bytes would need 6 (tensor pipe 48 %, issue
+// 36 %). Two blocks an SM, nothing spilled: 113 us against 117 before.
 #include "attn_rows.cuh"
 
 namespace voxcuda {

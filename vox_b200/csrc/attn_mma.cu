@@ -7,9 +7,10 @@
 // back as operands of mma.m16n8k16. Whole chunks serve as operands because the order of a product's summation index is
 // free: S^T = K Q^T sums over the head's elements, so lane (g, t) may supply of key g the 16-byte chunks t, t + 4, .. as they
 // lie in memory, if Q's operand takes the same chunks; and O^T = V^T P^T has V's elements as its rows, so lane (g, t) loads
-// the chunks g, g + 8 of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs two keys' halves with one byte permute. The weights turn from S^T's layout (lane: a key, two rows) to P^T's (lane: a row, two keys)
-// by one 8 x 8 transpose in registers. The softmax keeps one reference maximum a row for the warp, moved only when a score
-// exceeds it by 8 (base 2), so that the common step has one vote and no reduction.
+// the chunks g, g + 8 of keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs two keys' halves with one byte permute. The weights turn
+// from S^T's layout (lane: a key, two rows) to P^T's (lane: a row, two keys) by one 8 x 8 transpose in registers. The softmax
+// keeps one reference maximum a row for the warp, moved only when a score exceeds it by 8 (base 2), so that the common step
+// has one vote and no reduction.
 //
 // f32 activations keep f32 accuracy on the bf16 tensor cores: q and the weights are each cut into three bf16 parts (8 + 8 +
 // 8 significant bits), whose products with the bf16 keys and values are exact and accumulate in f32 in the same registers;

@@ -476,7 +476,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
 
 }  // namespace
 
-int attn_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int attn_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda
 

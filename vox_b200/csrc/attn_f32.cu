@@ -325,6 +325,6 @@ int attn_f32_launch(const AttnArgs &a, int head_dim, int dtype, int cache_dtype,
               : launch<bf, float, 128>(a, blocks, st, name);
 }
 
-int attn_f32_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int attn_f32_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda

@@ -394,6 +394,6 @@ int attn_mma_resident(int head_dim, int rows_blk, int dtype) {
                      [](auto core) { return rows_resident<decltype(core)>(); });
 }
 
-int attn_mma_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int attn_mma_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda

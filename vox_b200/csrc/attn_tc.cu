@@ -544,6 +544,6 @@ int attn_tc_launch(const AttnArgs &a, const vox_cuda_kv_cache &c, int64_t blocks
     return qt == 1 ? launch<128, 1>(a, mk, mv, blocks, st, name) : launch<128, 2>(a, mk, mv, blocks, st, name);
 }
 
-int attn_tc_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int attn_tc_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda

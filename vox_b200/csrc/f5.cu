@@ -1227,7 +1227,7 @@ int build(F5Plan &p, cudaStream_t user) {
 
 }  // namespace
 
-int f5_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int f5_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda
 

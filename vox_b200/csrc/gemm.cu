@@ -1325,7 +1325,7 @@ int gemm_q(bool q4, const void *w, const void *scale, int scale_dtype, const flo
     return rc;
 }
 
-int gemm_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int gemm_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda
 

@@ -54,7 +54,7 @@ struct GemmPlan {
 int gemm_plan(const void *x, int64_t ldx, const void *w, int64_t ldw, const GemmArgs &a, int epi, GemmPlan &plan, const char *name);
 // Launches a prepared GEMM on stream st.
 int gemm_run(const GemmPlan &plan, cudaStream_t st, const char *name);
-// Reads and clears the GEMM kernels' device error flag (bit 0: a bounded wait gave up).
-int gemm_take_device_error(unsigned int *flags);
+// Address of the GEMM kernels' device error flag on the current device (bit 0: a bounded wait gave up).
+int gemm_device_error_word(unsigned int **word);
 
 }  // namespace voxcuda

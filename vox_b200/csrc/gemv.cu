@@ -1158,7 +1158,7 @@ int gemv_entry(bool q4, const void *w, const void *scale, int scale_dtype, const
 
 }  // namespace
 
-int gemv_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int gemv_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda
 

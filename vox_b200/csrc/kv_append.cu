@@ -234,7 +234,7 @@ int paged_args(const vox_cuda_kv_cache *c, const vox_cuda_kv_batch *b, int64_t h
     return VOX_CUDA_OK;
 }
 
-int kv_append_take_device_error(unsigned int *flags) { return take_device_error(flags); }
+int kv_append_device_error_word(unsigned int **word) { return device_error_word(word); }
 
 }  // namespace voxcuda
 

@@ -832,6 +832,25 @@ int launch_softmax_pipe(const float *x, float *y, int64_t rows, int64_t n, float
                        : launch_row_pipe<SoftmaxOp<16>, kStages>(SoftmaxOp<16>{x, y, n, q_len, pos0, scale, qdiv}, rows, stage, st, name);
 }
 
+namespace {
+
+// The device error flags of all translation units, taken in one launch: each read and cleared in one atomic step on the
+// device (a flag raised by a kernel still running on another stream is either taken now or left set for the next read,
+// never lost).
+constexpr int kErrorWords = 9;
+struct ErrorWords {
+    unsigned int *at[kErrorWords];
+};
+__device__ unsigned int g_device_error_taken = 0;
+__global__ void take_device_error_kernel(const ErrorWords w) {
+    unsigned int v = 0;
+#pragma unroll
+    for (int i = 0; i < kErrorWords; ++i) v |= atomicExch(w.at[i], 0u);
+    g_device_error_taken = v;
+}
+
+}  // namespace
+
 }  // namespace voxcuda
 
 using namespace voxcuda;
@@ -844,11 +863,19 @@ extern "C" int vox_cuda_test_row_stall(int64_t row, uint64_t wait_limit_ns) {
 
 extern "C" int vox_cuda_device_error(unsigned int *flags) {
     VOX_REQUIRE(flags != nullptr, "vox_cuda_device_error: flags is NULL");
+    using WordOf = int (*)(unsigned int **);
+    constexpr WordOf words[kErrorWords] = {device_error_word,      gemv_device_error_word,    f5_device_error_word,
+                                           gemm_device_error_word, kv_append_device_error_word, attn_device_error_word,
+                                           attn_tc_device_error_word, attn_mma_device_error_word, attn_f32_device_error_word};
+    ErrorWords w;
+    bool ok = true;
+    for (int i = 0; i < kErrorWords; ++i) ok = ok && words[i](&w.at[i]) == VOX_CUDA_OK;
     unsigned int v = 0;
-    if (take_device_error(&v) != VOX_CUDA_OK || gemv_take_device_error(&v) != VOX_CUDA_OK || f5_take_device_error(&v) != VOX_CUDA_OK ||
-        gemm_take_device_error(&v) != VOX_CUDA_OK || kv_append_take_device_error(&v) != VOX_CUDA_OK ||
-        attn_take_device_error(&v) != VOX_CUDA_OK || attn_tc_take_device_error(&v) != VOX_CUDA_OK ||
-        attn_mma_take_device_error(&v) != VOX_CUDA_OK || attn_f32_take_device_error(&v) != VOX_CUDA_OK) {
+    if (ok) {  // on the legacy default stream, so it follows the work of every blocking stream
+        take_device_error_kernel<<<1, 1>>>(w);
+        ok = cudaGetLastError() == cudaSuccess && cudaMemcpyFromSymbol(&v, g_device_error_taken, sizeof(v)) == cudaSuccess;
+    }
+    if (!ok) {
         const cudaError_t e = cudaGetLastError();
         return set_error(VOX_CUDA_ERR_DEVICE, std::string("vox_cuda_device_error: ") + cudaGetErrorString(e));
     }

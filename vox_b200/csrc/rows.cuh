@@ -50,15 +50,14 @@ int launch_reduce_pipe(const void *x, float *out, int64_t rows, int64_t n, int o
 int launch_softmax_pipe(const float *x, float *y, int64_t rows, int64_t n, float scale, int64_t q_len, int64_t pos0,
                         cudaStream_t st);
 
-// Reads and clears the quantized GEMV's device error flag into *flags (gemv.cu); VOX_CUDA_OK or VOX_CUDA_ERR_DEVICE.
-int gemv_take_device_error(unsigned int *flags);
-// The same for the F5 step's attention kernel (f5.cu).
-int f5_take_device_error(unsigned int *flags);
-// And for the paged-cache operators (kv_append.cu, attn.cu, attn_tc.cu, attn_mma.cu, attn_f32.cu).
-int kv_append_take_device_error(unsigned int *flags);
-int attn_take_device_error(unsigned int *flags);
-int attn_tc_take_device_error(unsigned int *flags);
-int attn_mma_take_device_error(unsigned int *flags);
-int attn_f32_take_device_error(unsigned int *flags);
+// Address of the device error flag of another translation unit's kernels on the current device (gemv.cu, f5.cu, kv_append.cu,
+// attn.cu, attn_tc.cu, attn_mma.cu, attn_f32.cu); VOX_CUDA_OK or VOX_CUDA_ERR_DEVICE.
+int gemv_device_error_word(unsigned int **word);
+int f5_device_error_word(unsigned int **word);
+int kv_append_device_error_word(unsigned int **word);
+int attn_device_error_word(unsigned int **word);
+int attn_tc_device_error_word(unsigned int **word);
+int attn_mma_device_error_word(unsigned int **word);
+int attn_f32_device_error_word(unsigned int **word);
 
 }  // namespace voxcuda

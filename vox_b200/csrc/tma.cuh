@@ -19,7 +19,7 @@ namespace voxcuda {
 
 // Device-side error flag of the pipelines (a bit set by a kernel that gave up a wait). The library is built without
 // relocatable device code, so every translation unit that includes this header has its own flag; each of them
-// exposes it through take_device_error() and vox_cuda_device_error() gathers them all.
+// gives its address (device_error_word()) and vox_cuda_device_error() reads and clears them all in one launch.
 static __device__ unsigned int g_device_error = 0;
 constexpr unsigned int kDevErrTimeout = 1u;
 // A wait gives up after this much time on the GPU's global timer (ns), read every 32 polls (each try_wait may also
@@ -176,20 +176,9 @@ int launch_row_pipe(const Op &op, int64_t rows, uint32_t stage_bytes, cudaStream
     return check_launch(name);
 }
 
-// The flag read and cleared in one atomic step on the device (a flag raised by a kernel still running on another
-// stream is either taken now or left set for the next read, never lost).
-static __device__ unsigned int g_device_error_taken = 0;
-static __global__ void take_device_error_kernel() { g_device_error_taken = atomicExch(&g_device_error, 0u); }
-
-// Reads and clears this translation unit's device error flag (host side; the legacy default stream, so it follows
-// the work of every blocking stream). VOX_CUDA_OK or VOX_CUDA_ERR_DEVICE.
-static inline int take_device_error(unsigned int *flags) {
-    unsigned int v = 0;
-    take_device_error_kernel<<<1, 1>>>();
-    if (cudaGetLastError() != cudaSuccess || cudaMemcpyFromSymbol(&v, g_device_error_taken, sizeof(v)) != cudaSuccess)
-        return VOX_CUDA_ERR_DEVICE;
-    *flags |= v;
-    return VOX_CUDA_OK;
+// Address of this translation unit's device error flag on the current device. VOX_CUDA_OK or VOX_CUDA_ERR_DEVICE.
+static inline int device_error_word(unsigned int **word) {
+    return cudaGetSymbolAddress(reinterpret_cast<void **>(word), g_device_error) == cudaSuccess ? VOX_CUDA_OK : VOX_CUDA_ERR_DEVICE;
 }
 
 // Test hook (host side): sets this translation unit's wait limit (ns; 0 restores the default) and stalled row.

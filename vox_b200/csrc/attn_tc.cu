@@ -90,10 +90,11 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 // 2^x for x <= 64 or so on the multiply-add pipe (two elements), beside the 16 results a clock of the special-function unit:
 // x = n + f, n the nearest integer (from the low bits of x + 1.5 2^23), 2^f by a cubic whose relative error on
 // [-1/2, 1/2] is below 7.5e-5 (a least-maximum fit made for this kernel; the weights are rounded to bf16 next, 2^-8), times 2^n
-// built from its exponent bits. Below -126 (masked scores too) it gives 2^-126; NaN stays NaN.
+// built from its exponent bits. n = -127 has the bits of 0, so below -126.5 (masked scores too) it gives exactly 0, as
+// ex2_approx does; NaN stays NaN.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
     const float2 t = add2(x, bc2(12582912.0f));
     const float2 f = add2(x, fma2(t, bc2(-1.0f), bc2(12582912.0f)));
     float2 p = fma2(bc2(0.05517132f), f, bc2(0.24261054f));
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(tc_threads(QT), QT == 1 ? 2 : 1)
             tc_fence_after();
         }
         const float2 ls = add2(add2(l2[0], l2[1]), add2(l2[2], l2[3]));
-        const float l = ref == -INFINITY && ls.x + ls.y < 1.0f ? 0.f : ls.x + ls.y;  // a row that saw no key (a NaN sum stays)
+        const float l = ls.x + ls.y;  // of a row that saw no key: exactly 0
         const int h = j.kvh * a.p.group + (live ? rr - i_tok * a.p.group : 0);
         const int64_t tok = j.tok0 + i_tok;
         const int64_t slot = (tok * a.p.heads + h) * a.splits + j.split;

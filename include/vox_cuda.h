@@ -311,7 +311,9 @@ typedef struct vox_cuda_kv_cache {
  *   kv_len     [seqs]: rows of each sequence in the cache, its new tokens included
  *   q_start    [seqs + 1]: first token of each sequence among the `tokens` rows of qkv / q / out, ascending; or NULL:
  *              every sequence has tokens / seqs of them
- *   tokens:    new tokens of all sequences together
+ *   tokens:    new tokens of all sequences together (0 is no error; without a sequence it has to be 0). Rows from
+ *              q_start[seqs] on belong to no sequence: the attention leaves their results undefined, the append skips them and
+ *              sets VOX_CUDA_DEVERR_RANGE
  *   max_q, max_kv: bounds of a sequence's new tokens and of kv_len. They size the launch only: longer sequences are still
  *              computed whole, more slowly. 0: tokens, and table_width * page_size.
  * Token i of sequence b stands at position kv_len[b] - q_len[b] + i. Lengths and page numbers are checked on the device:

@@ -402,7 +402,7 @@ int attn_run(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, con
     VOX_REQUIRE(is_act_dtype(dtype), std::string(name) + ": dtype must be f32 or bf16");
     VOX_REQUIRE(window >= 0 && prefix_len >= 0 && prefix_len < (int64_t(1) << 30), std::string(name) + ": window or prefix_len out of range");
     if (want) *want = 0;
-    if (batch->seqs == 0 || batch->tokens == 0) return VOX_CUDA_OK;
+    if (batch->tokens == 0) return VOX_CUDA_OK;
     const int hd = cache->head_dim;
     const int64_t max_q = batch->q_start == nullptr ? a.p.q_per : batch->max_q > 0 && batch->max_q < batch->tokens ? batch->max_q : batch->tokens;
     const int64_t max_kv = batch->max_kv > 0 && batch->max_kv < a.p.cap ? batch->max_kv : a.p.cap;

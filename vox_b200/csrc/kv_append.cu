@@ -218,7 +218,8 @@ int paged_args(const vox_cuda_kv_cache *c, const vox_cuda_kv_batch *b, int64_t h
                 std::string(name) + ": bad batch shape");
     VOX_REQUIRE(b->tokens * heads < (int64_t(1) << 31) && int64_t(b->table_width) * c->page_size <= (int64_t(1) << 30),
                 std::string(name) + ": sizes out of range");
-    if (b->seqs == 0 || b->tokens == 0) return VOX_CUDA_OK;
+    VOX_REQUIRE(b->seqs > 0 || b->tokens == 0, std::string(name) + ": tokens without a sequence");
+    if (b->tokens == 0) return VOX_CUDA_OK;
     VOX_REQUIRE(c->k && c->v && (b->page_table || b->table_width == 0) && b->kv_len, std::string(name) + ": NULL pointer");
     VOX_REQUIRE(aligned16(c->k) && aligned16(c->v), std::string(name) + ": the cache must be 16-byte aligned");
     VOX_REQUIRE(b->q_start || b->tokens % b->seqs == 0, std::string(name) + ": without q_start the tokens must be a multiple of seqs");
@@ -247,7 +248,7 @@ extern "C" int vox_cuda_kv_append(const vox_cuda_kv_cache *cache, const vox_cuda
     const int rc = paged_args(cache, batch, heads, "vox_cuda_kv_append", a.p);
     if (rc != VOX_CUDA_OK) return rc;
     VOX_REQUIRE(is_act_dtype(dtype), "vox_cuda_kv_append: dtype must be f32 or bf16");
-    if (batch->seqs == 0 || batch->tokens == 0) return VOX_CUDA_OK;
+    if (batch->tokens == 0) return VOX_CUDA_OK;
     VOX_REQUIRE(qkv && cs && q, "vox_cuda_kv_append: NULL pointer");
     const int hd = cache->head_dim;
     const int64_t el = 16 / dtype_size(dtype), units = heads + 2 * int64_t(cache->kv_heads);

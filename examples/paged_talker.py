@@ -33,13 +33,24 @@ class Pool:
         self.table = torch.zeros((streams, width), dtype=torch.int32)
 
     def take(self, n: int) -> list[int]:
+        if n > len(self.free):
+            raise RuntimeError(f"the pool has {len(self.free)} free pages, {n} are needed")
         return [self.free.pop() for _ in range(n)]
 
     def grow(self, lens) -> None:
         for b, n in enumerate(lens):
+            if n > self.table.shape[1] * self.page:
+                raise RuntimeError(f"stream {b} has {n} rows, its page table holds {self.table.shape[1]} pages of {self.page}")
             while len(self.of[b]) * self.page < n:
-                self.table[b, len(self.of[b])] = self.free[-1]
-                self.of[b].append(self.free.pop())
+                self.of[b] += self.take(1)
+                self.table[b, len(self.of[b]) - 1] = self.of[b][-1]
+
+
+def sizes(texts, steps: int, voice: int, page: int) -> tuple[int, int, int]:
+    """(pages of the pool, pages of a stream's table, positions) that texts of these lengths need with `steps` more tokens each
+    behind a voice prompt."""
+    need = [-(-(n + steps) // page) for n in texts]
+    return sum(need) + -(-voice // page), max(need), voice + max(texts) + steps
 
 
 class Talker:
@@ -83,8 +94,9 @@ def run(streams=8, steps=16, layers=2, dtype=torch.bfloat16, voice=100, page=16,
     with the inputs that led to them (the model's own output is the next input: a stand-in for sampling)."""
     g = torch.Generator().manual_seed(seed + 1)
     texts = [5 + int(x) for x in torch.randint(0, 40, (streams,), generator=g)]
-    t = Talker(layers=layers, dtype=dtype, seed=seed, page=page, pages=streams * 8 + 32)
-    pool = Pool(t.cache[0].pages, page, streams, 64)
+    pages, width, positions = sizes(texts, steps, voice, page)
+    t = Talker(layers=layers, dtype=dtype, seed=seed, page=page, pages=pages, positions=positions)
+    pool = Pool(pages, page, streams, width)
     dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
     hidden = lambda n: torch.randn((n, t.dim), generator=g).to(dtype)  # noqa: E731
     # the voice prompt, once
@@ -103,6 +115,7 @@ def run(streams=8, steps=16, layers=2, dtype=torch.bfloat16, voice=100, page=16,
                          prefix=prefix)
     x = out_text[torch.tensor(starts[1:], device="cuda") - 1]
     seen = []
+    torch.cuda.synchronize()  # the voice and the texts are not part of a step
     t0 = time.perf_counter()
     for _ in range(steps):
         lens = [n + 1 for n in lens]
@@ -122,4 +135,4 @@ if __name__ == "__main__":
     ap.add_argument("--dtype", choices=["bf16", "f32"], default="bf16")
     args = ap.parse_args()
     r = run(args.streams, args.steps, args.layers, torch.bfloat16 if args.dtype == "bf16" else torch.float32)
-    print(f"{args.streams} streams x {args.steps} steps behind one voice prompt: {r['seconds'] / args.steps * 1e3:.2f} ms a step")
+    print(f"{args.streams} streams x {args.steps} steps behind one voice prompt: {r['seconds'] / max(args.steps, 1) * 1e3:.2f} ms a step")

@@ -329,7 +329,10 @@ typedef struct vox_cuda_kv_batch {
  * rotates q and k (rotate-half) at the token's position, writes q and the token's K and V rows into its sequence's pages.
  *   qkv [tokens][heads*hd + 2*kv_heads*hd], row stride qkv_stride elements; q [tokens][heads*hd], row stride q_stride;
  *   both in `dtype` (f32 or bf16); the cache rows are rounded once to the cache's dtype
- *   cs: f32 [cs_rows][hd/2][2], the vox_cuda_rope_table of positions 0 .. cs_rows-1 (every position needs its row);
+ *   cs: f32 [cs_rows][hd/2][2], the vox_cuda_rope_table of positions 0 .. cs_rows-1 (every position needs its row). A token is
+ *   rotated by the table's row of its own position, kv_len - q_len + i, which does not count a shared prefix: for tokens that
+ *   vox_cuda_attn_prefix puts behind prefix_len rows pass the table from row prefix_len on (cs + prefix_len * hd, with
+ *   cs_rows - prefix_len rows);
  *   q_norm_w / k_norm_w: f32 [hd] or NULL; eps their epsilon
  * Arithmetic as vox_cuda_qkv_rope (with f32 in and out and no head norms bit-identical to rope_apply, kernels.cpp:740-757).
  * A token whose position has no page or no table row is skipped and sets VOX_CUDA_DEVERR_RANGE. No two tokens
@@ -356,7 +359,8 @@ VOX_CUDA_API int vox_cuda_attn_paged(const vox_cuda_kv_cache *cache, const vox_c
 
 /* The same attention for a batch whose sequences all stand behind one shared prefix (a voice prompt): every token sees the
  * prefix_len rows behind prefix_pages (device, ceil(prefix_len / page_size) page numbers), then its own sequence's rows as
- * above (kv_len counts the sequence's own rows). The prefix is read for the rows of the whole batch together, unless the call
+ * above (kv_len counts the sequence's own rows). The prefix comes first in position, which the keys' and queries' rotation has to
+ * say: append them with the rotation table from row prefix_len on (vox_cuda_kv_append). The prefix is read for the rows of the whole batch together, unless the call
  * is so small, or its texts so long, that a walk of its own costs more than reading it for every sequence; the two parts'
  * softmax statistics are joined exactly. prefix_len 0 is vox_cuda_attn_paged. */
 VOX_CUDA_API int vox_cuda_attn_prefix(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, const int32_t *prefix_pages,

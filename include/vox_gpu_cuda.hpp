@@ -94,7 +94,8 @@ bool gpu_kv_append(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batc
 // rows; workspace of gpu_attn_workspace bytes.
 bool gpu_attn_paged(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const void *q, void *out, int64_t heads, float scale,
                     int64_t window, void *workspace, size_t workspace_bytes, int dtype = VOX_CUDA_F32, void *stream = nullptr);
-// The same behind one prefix that all sequences share (a voice prompt).
+// The same behind one prefix that all sequences share (a voice prompt). It comes first in position: the tokens behind it are appended
+// with the rotation table from row prefix_len on (cs + prefix_len * hd, cs_rows - prefix_len).
 bool gpu_attn_prefix(const vox_cuda_kv_cache &cache, const vox_cuda_kv_batch &batch, const int32_t *prefix_pages, int64_t prefix_len,
                      const void *q, void *out, int64_t heads, float scale, void *workspace, size_t workspace_bytes,
                      int dtype = VOX_CUDA_F32, void *stream = nullptr);

@@ -4,8 +4,12 @@ what their documents say."""
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 from tests.test_paged_host import batch, cache, size, v  # noqa: F401
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 def test_tokens_of_no_sequence_are_refused(v):  # noqa: F811
@@ -20,3 +24,21 @@ def test_tokens_of_no_sequence_are_refused(v):  # noqa: F811
                    L.vox_cuda_kv_append(C, B, 4096, 512, None, None, 4096, 64, 8192, 256, 4, 1e-6, 1, None)):
             assert rc == -6
             assert "without a sequence" in L.vox_cuda_last_error().decode()
+
+
+def test_documents_say_which_rotation_stands_behind_a_prefix(v):  # noqa: F811
+    """The append rotates by the row in the sequence's own pages, so behind a shared prefix its table starts at row prefix_len.
+    Whoever calls the two operators finds that at each of them, and the documented call does it."""
+    header = (ROOT / "include" / "vox_cuda.h").read_text()
+    at = {n: header.index("int " + n + "(") for n in ("vox_cuda_kv_append", "vox_cuda_attn_paged", "vox_cuda_attn_prefix", "vox_cuda_attn_workspace")}
+    before = {"vox_cuda_kv_append": header.rindex("/*", 0, at["vox_cuda_kv_append"]), "vox_cuda_attn_prefix": at["vox_cuda_attn_paged"]}
+    for n, start in before.items():
+        text = " ".join(header[start:at[n]].replace("*", " ").split())
+        assert "from row prefix_len on" in text, n
+    seam = (ROOT / "include" / "vox_gpu_cuda.hpp").read_text()
+    assert "from row prefix_len on" in " ".join(seam[:seam.index("bool gpu_attn_prefix(")].replace("//", " ").split())
+    for f in (v.PagedKV.append, v.PagedKV.attend_prefix):
+        assert "cs[prefix_len:]" in f.__doc__, f
+    guide = (ROOT / "INTEGRATION.md").read_text()
+    calls = re.findall(r"gpu_kv_append\(([^;]*)\);", guide)
+    assert calls and all("prefix_len" in c for c in calls)

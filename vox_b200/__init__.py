@@ -616,7 +616,8 @@ class PagedKV:
                q=None) -> torch.Tensor:
         """qkv_rope for a ragged batch: splits the fused projection qkv [tokens][(heads + 2 kv_heads) head_dim], head-
         RMSNorms and rotates q and k at each token's position, writes K and V into the sequences' pages and returns q
-        [tokens][heads * head_dim] (qkv's dtype). cs: rope_table(inv_freq, 0, n) of all positions in use."""
+        [tokens][heads * head_dim] (qkv's dtype). cs: rope_table(inv_freq, 0, n) of all positions in use; a token's position is
+        its row in its own sequence, so for tokens behind a shared prefix (attend_prefix) pass cs[prefix_len:]."""
         hd = self.head_dim
         dt, tokens, stride, _ = self._rows(qkv, "qkv", (heads + 2 * self.kv_heads) * hd)
         csp, qnp, knp = self._vec(cs, "cs"), self._vec(q_norm_w, "q_norm_w"), self._vec(k_norm_w, "k_norm_w")
@@ -646,7 +647,8 @@ class PagedKV:
     def attend_prefix(self, q, prefix_pages, prefix_len: int, page_table, kv_len, q_start=None, max_q: int = 0, max_kv: int = 0,
                       scale: float | None = None, out=None) -> torch.Tensor:
         """attend() for sequences that all stand behind one shared prefix: every token sees the prefix_len rows behind
-        prefix_pages (int32), read for the whole batch together, and then its own sequence's rows as in attend()."""
+        prefix_pages (int32), read for the whole batch together, and then its own sequence's rows as in attend(). The prefix
+        comes first in position: append the sequences' tokens with cs[prefix_len:]."""
         if not (isinstance(prefix_pages, torch.Tensor) and prefix_pages.dtype is torch.int32 and prefix_pages.get_device() == self._dev and
                 prefix_pages.dim() == 1 and prefix_pages.is_contiguous()):
             raise VoxCudaError(-6, "prefix_pages must be a contiguous int32 tensor on the cache's device")

@@ -367,8 +367,11 @@ VOX_CUDA_API int vox_cuda_attn_prefix(const vox_cuda_kv_cache *cache, const vox_
                                       int64_t prefix_len, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                                       int64_t heads, float scale, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Bytes of workspace that vox_cuda_attn_paged (prefix_len 0) or vox_cuda_attn_prefix needs for this cache and batch shape
- * (seqs, tokens, max_q, max_kv; the arrays are not read). */
+/* Bytes of workspace that vox_cuda_attn_paged (prefix_len 0) or vox_cuda_attn_prefix needs for this cache and batch
+ * shape: pass the description that the call will get, since seqs, tokens, max_q and max_kv, whether q_start is NULL,
+ * table_width * page_size (where max_kv is 0 or above it) and the cache's types and heads all count, and with the device of the call as the
+ * current device (its number of SMs and how many blocks they hold count too). The arrays are not read, but as in the call only
+ * q_start may be NULL. Nothing is launched. */
 VOX_CUDA_API int vox_cuda_attn_workspace(const vox_cuda_kv_cache *cache, const vox_cuda_kv_batch *batch, int64_t prefix_len,
                                          int64_t heads, int64_t window, int dtype, size_t *bytes);
 

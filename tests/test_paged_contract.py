@@ -42,3 +42,19 @@ def test_documents_say_which_rotation_stands_behind_a_prefix(v):  # noqa: F811
     guide = (ROOT / "INTEGRATION.md").read_text()
     calls = re.findall(r"gpu_kv_append\(([^;]*)\);", guide)
     assert calls and all("prefix_len" in c for c in calls)
+
+
+def test_size_query_names_all_that_it_depends_on(v):  # noqa: F811
+    """The bytes follow from the whole description of the batch: with and without token offsets they differ, and so they do with the
+    table's width where max_kv is left to it."""
+    c = cache(v)
+    big = dict(tokens=40, seqs=10, table_width=400, table_stride=400)
+    need = [size(v, c, batch(**big), prefix=900), size(v, c, batch(q_start=4096, **big), prefix=900),
+            size(v, c, batch(**{**big, "table_width": 1}), prefix=900)]
+    assert all(rc == 0 for rc, _ in need) and len({n for _, n in need}) > 1
+    header = (ROOT / "include" / "vox_cuda.h").read_text()
+    end = header.index("int vox_cuda_attn_workspace(")
+    text = " ".join(header[header.rindex("/*", 0, end):end].replace("*", " ").split())
+    for word in ("q_start", "table_width", "current device", "not read", "NULL"):
+        assert word in text, word
+    assert "host arithmetic only" not in (ROOT / "INTEGRATION.md").read_text()

@@ -75,3 +75,26 @@ def test_values_of_later_rows_do_not_leak_in_one_tile_blocks(vox, hd):
         want, mag, big = attention64(bt, q, 8, hd ** -0.5)
         keep = [b * n + i for b in range(40) for i in range(n - late)]
         check_rows(got, want, mag, big, BF16, BF16, n + prefix, keep)
+
+
+@pytest.mark.parametrize("act,cache", KINDS, ids=IDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,seqs", [(1, 2), (1, 200), (5, 3), (70, 3), (200, 2), (30, 40)])
+def test_pages_far_in_front_of_a_window_are_given_away(vox, act, cache, hd, n, seqs):
+    """Rows 128 and more in front of the first row that a sequence's tokens see are never read: their page table entries name no
+    page, and nothing is reported. (The 127 rows between hold finite values that no token sees.)"""
+    window, page = 50, 16
+    lens = [(n, n + 600 + 37 * b % 300) for b in range(seqs)]
+    bt = Batch(lens, 4, hd, page, cache, seed=n + hd)
+    q = queries(bt, 8, act)
+    want, mag, big = attention64(bt, q, 8, hd ** -0.5, window)
+    kv = bt.handle(vox)
+    for b, (_, k) in enumerate(lens):
+        gone = max(k - n + 1 - window - 127, 0) // page  # whole pages of such rows
+        assert gone > 0
+        bt.table[b, :gone] = -1
+    table, kv_len, q_start = bt.dev(uniform=True)
+    for qs, mq, mkv in ((None, 0, 0), (bt.q_start.cuda(), n, max(k for _, k in lens)), (bt.q_start.cuda(), 0, 0)):
+        got = kv.attend(q.cuda(), table, kv_len, q_start=qs, max_q=mq, max_kv=mkv, window=window)
+        check_rows(got, want, mag, big, act, cache, 1100, slice(None))
+    assert vox.device_error() == 0

@@ -19,7 +19,9 @@
  *   - "Activations" follow the call's dtype (VOX_CUDA_F32 or VOX_CUDA_BF16). Learned weight vectors that Vox
  *     holds as `const float *` (norm weights and biases, Snake alpha/beta) are always f32. Per-batch
  *     modulation vectors of adaLN (shift/scale/gate) follow the call's dtype.
- *   - Arithmetic is f32 for every dtype; bf16 outputs are rounded to nearest-even once, at the store.
+ *   - Arithmetic is f32 for every dtype; bf16 outputs are rounded to nearest-even once, at the store. Operators that round
+ *     something between say so at their entry: vox_cuda_attn_paged and vox_cuda_attn_prefix with bf16 activations on a
+ *     bf16 cache round the softmax weights to bf16, and the tensor-core GEMMs and the F5 DiT step their operands.
  *   - Reductions use a fixed order (no floating-point atomics): results are bitwise reproducible run to run.
  */
 #ifndef VOX_CUDA_H

@@ -41,13 +41,15 @@ __device__ __forceinline__ void halve(float (&s)[N], int lane) {
 // and 4 rows, 369 against 227 at 8.) The rows' references are the warp's and move only when a score exceeds one by 8 (base 2):
 // the common step has one vote. Every warp takes each kRowsWarps-th run of KPI keys; from four rows on, the next step's K is
 // loaded while this one's weights and products are worked on (without it 169 us for 139, 297 for 225).
-// At that size, 8 heads of 128: 2 rows 130 us (6.3 TB/s), 4 rows 139, 8 rows 192 (bound by the exchanges and additions). One token
-// over 650 keys takes 8.4 us in a graph: latency (its 5 MB would need 0.8).
+// At that size, 8 heads of 128: 1 row 135 us (5.9 TB/s), 2 rows 126 (6.3), 4 rows 139, 8 rows 186 (4.3, bound by the exchanges and
+// additions). One token over 650 keys takes 8.4 us in a graph: latency (its 5 MB would need 0.8).
 template <typename QT, int HD_, int R>
 struct VecCore {
     using Q = QT;
     // of 8 rows, three blocks an SM spill 150 bytes and still pay in long runs (192 us against 225 at the size above, 14 heads on
-    // 2 of 64 55 against 63), but not in small calls (26 against 24 at 8 sequences of 1000 keys)
+    // 2 of 64 55 against 63), but not in small calls (26 against 24 at 8 sequences of 1000 keys). Four blocks an SM of 2 and 4 rows
+    // spill too: 28-80 bytes in the stream frame, and 36-72 in the cluster frame, which never has as many on an SM and would not
+    // need the bound (what that costs there is not measured).
     static constexpr int HD = HD_, RB = R, kMinBlocks = R <= 4 ? 4 : 2, kStreamBlocks = R <= 4 ? 4 : 3;
     static constexpr size_t kSmem = 0;
     struct State {};

@@ -16,8 +16,9 @@
 // QT 1: the same with one row tile, stages of 64 keys and half of the tensor memory, so that two blocks share an SM (many
 // short texts; the rule is in attn.cu). Below, roles and columns are QT 2's.
 //
-// Measured: one prompt of 8192 tokens, 16 query heads on 8 of 128, 231 us in a graph: 1190 TFLOP/s of the causal half, 0.71 of
-// what a bare product reaches. Bound by the softmax, some 1610 clocks per 64 keys of both row tiles (exponentials, their
+// Measured: one prompt of 8192 tokens, 16 query heads on 8 of 128, 237 us in the first 20 ms from idle, at 1965 MHz (1160 TFLOP/s of
+// the causal half, 0.70 of the burst rate of a bare product), and 274 us when run on end for two seconds, at 1605 MHz under the
+// 1000 W cap (1000 TFLOP/s, 0.72 of the sustained rate); 7 ragged prompts 210 and 239 us (1725 MHz). Bound by the softmax, some 1610 clocks per 64 keys of both row tiles (exponentials, their
 // latency, and the tensor-memory loads before them) where the products need half; every block adds some 6 us before its
 // first and after its last product. One S buffer a row tile and steps of 128 keys, so that the products stand in the softmax's
 // path: 249 us against 210 at 7 ragged prompts, 56 against 50 at 24 texts behind one prefix.
@@ -132,7 +133,9 @@ __device__ __forceinline__ void tc_job(const AttnArgs &a, uint32_t blk, TcJob &o
     } else {
         const uint32_t t0 = a.osdiv.div(y);
         const int s = int(y - t0 * uint32_t(a.own_splits));
-        int t = a.own_tiles - 1 - int(t0), b = -1, n = 0, tile = 0;  // the last rows, which see most keys, first
+        // the list of all sequences' row tiles from its end: within a sequence the last rows, which see most keys, first, but the
+        // sequences in descending order whatever their lengths
+        int t = a.own_tiles - 1 - int(t0), b = -1, n = 0, tile = 0;
         if (a.p.q_start == nullptr) {
             const int per = (a.p.q_per * a.p.group + a.tc_rows - 1) / a.tc_rows;
             b = t / per;

@@ -349,10 +349,12 @@ VOX_CUDA_API int vox_cuda_kv_append(const vox_cuda_kv_cache *cache, const vox_cu
  * head h / (heads / kv_heads). Prompts and single tokens alike (q_len 0, 1 or more a sequence, mixed in a call).
  *   q, out [tokens][heads][hd], row strides q_stride / out_stride elements, `dtype` f32 or bf16; out must not overlap q
  * A token that sees no key gives zeros. Cache rows at or past kv_len are never used, whatever they hold; the rows below it
- * must be finite, and their values so small that 256 times the sum of |v| over a sequence's rows is a finite f32 (weights are up to
- * 2^8 before their sum divides them). A key that a token does not see has the weight 0. With a window, rows 128 and more in front of
- * the first row that a sequence's tokens see are not read, and their pages may be given away. Scores, softmax statistics and sums are f32. bf16 activations on a bf16 cache: the weights are rounded to
- * bf16 for the product with v (2^-8 relative). Every other pair of types keeps f32 accuracy (about 1e-6): few rows on an f32
+ * must be finite, and their values so small that 256 times the sum of |v| over a sequence's rows is a finite f32 (the weights
+ * are up to 2^8 before their sum divides them). A key that a token does not see has the weight 0. With a window, rows 128 and
+ * more in front of the first row that a sequence's tokens see are not read, and their pages may be given away; the call is
+ * still cut by max_kv, so a short window over long sequences is served, but not at its floor.
+ * Scores, softmax statistics and sums are f32. bf16 activations on a bf16 cache: the weights are rounded to bf16 for the
+ * product with v (2^-8 relative). Every other pair of types keeps f32 accuracy (about 1e-6): few rows on an f32
  * cache run on the CUDA cores, the rest on the tensor cores with operands cut into parts whose products are exact to 2^-21.
  * Results are identical run to run. workspace: vox_cuda_attn_workspace bytes of scratch, 256-byte aligned (NULL where that
  * says 0), not shared by calls that can overlap. Replaces attention.comp:1-45 and the attention of transformer_forward

@@ -296,7 +296,9 @@ AttnShape attn_shape(const PagedArgs &p, int head_dim, int dtype, bool bf16_cach
     // Blocks of one row tile, two an SM, where no sequence has more and there are more than one an SM: a block's start and end
     // lie behind the other's walk: 24 texts of 128 rows behind 1003 28.8 us (37.8 in blocks of two tiles), of 64 29.2 (36.3), 64 prompts
     // of 120 rows 28.9 (41.3). With fewer blocks their stages of half the size cost more: 64 rows on each of 16 sequences of 2000
-    // keys 49 against 35; and so do long rows (8192 tokens 271 against 234: every tile of keys is read for half as many rows)
+    // keys 49 against 35; and so do longer rows, since every tile of keys is read for half as many: 24 texts of 7-150 tokens behind
+    // 1003 54.4 against 49.4, of 100-150 60.4 against 53.9, 12 of 7-150 33.8 against 27.4 (48 of them 107.5 both ways), one prompt of
+    // 8192 tokens 271 against 234
     s.tc_half = s.own_tc && rows <= 128 && tiles(128) * p.kv_heads > sms;
     // The prefix in front of each text's own keys in the same block, without a join; or apart, for the rows of all texts
     // together, which fill their row tiles: apart if that spares an SM more than ten tiles of 128 keys, or the texts are short.

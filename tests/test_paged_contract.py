@@ -7,6 +7,9 @@ import ctypes
 import re
 from pathlib import Path
 
+import pytest
+import torch
+
 from tests.test_paged_host import batch, cache, size, v  # noqa: F401
 
 ROOT = Path(__file__).resolve().parents[1]
@@ -58,3 +61,14 @@ def test_size_query_names_all_that_it_depends_on(v):  # noqa: F811
     for word in ("q_start", "table_width", "current device", "not read", "NULL"):
         assert word in text, word
     assert "host arithmetic only" not in (ROOT / "INTEGRATION.md").read_text()
+
+
+def test_bounds_that_do_not_fit_are_refused_in_the_library_s_manner(v):  # noqa: F811
+    """max_q and max_kv are 32-bit numbers: others are an argument error of the library, not of the packing below it."""
+    kv = v.PagedKV.__new__(v.PagedKV)
+    kv._dev = -1  # host tensors stand in for a batch: nothing is called
+    table, lens = torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    assert len(kv._batch(2, table, lens, None, 1, 2 ** 31 - 1)) == 56
+    for mq, mkv in ((2 ** 31, 0), (0, 2 ** 40), (0, -2 ** 31 - 1), (1.5, 0), (0, None)):
+        with pytest.raises(v.VoxCudaError, match="max_q and max_kv"):
+            kv._batch(2, table, lens, None, mq, mkv)

@@ -578,7 +578,10 @@ class PagedKV:
                 raise VoxCudaError(-6, "page_table [seqs][width], kv_len [seqs] and q_start [seqs + 1] must agree")
         if kv_len.numel() != seqs:
             raise VoxCudaError(-6, "page_table [seqs][width], kv_len [seqs] and q_start [seqs + 1] must agree")
-        return _pack_batch(page_table.data_ptr(), kv_len.data_ptr(), start, stride[0], tokens, seqs, width, max_q, max_kv)
+        try:
+            return _pack_batch(page_table.data_ptr(), kv_len.data_ptr(), start, stride[0], tokens, seqs, width, max_q, max_kv)
+        except struct.error:
+            raise VoxCudaError(-6, f"max_q and max_kv must be integers below 2^31, got {max_q!r} and {max_kv!r}") from None
 
     def _rows(self, t, name, width):
         """(dtype, tokens, row stride, elements a token) of activations [tokens][...] contiguous within a token."""
